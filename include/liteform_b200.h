@@ -409,6 +409,93 @@ int lf_row_stats(const int64_t* indptr /*[dev]*/, int64_t row_begin, int64_t row
 int lf_shard_rows(const int64_t* indptr /*[dev]*/, int64_t num_rows, int32_t num_shards,
                   int64_t* splits /*[dev] G+1, written asynchronously on `stream`*/, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Operators of a layer around the CSR product (no counterpart in the reference, whose product ends
+ * with C = A * B, format_algos.py:1660-1755): the norm that makes the rows of B, the product with
+ * the end of the layer in its epilogue, and the gradients of both.
+ *
+ * Types are LF_DTYPE_*; LF_DTYPE_E4M3 is the 8-bit float with 4 exponent and 3 mantissa bits (no
+ * infinity, largest value 448), always with one float32 scale per row: the row stands for
+ * scale * its stored values.  Sums, statistics and activations are float32, every output is
+ * rounded once, to nearest even.  Strides (ld...) are in elements; rows may start anywhere their
+ * element type allows, but rows on 16-byte boundaries (address and stride) move faster.  Results
+ * do not depend on the order in which thread blocks run: the same call gives the same bits.
+ * ------------------------------------------------------------------------------------------- */
+#define LF_DTYPE_E4M3 3
+#define LF_ACT_NONE 0
+#define LF_ACT_RELU 1        /* max(z, 0); NaN stays NaN                                   */
+#define LF_ACT_SILU 2        /* z / (1 + exp(-z))                                          */
+#define LF_ACT_GELU 3        /* z (1 + erf(z / sqrt 2)) / 2                                */
+#define LF_ACT_GELU_TANH 4   /* z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2            */
+
+/* What follows the sum of a row; all zero: nothing. */
+typedef struct lf_epilogue {
+  const void* bias;          /* [dev] N values, or NULL                                    */
+  const void* residual;      /* [dev] one row per row of C, or NULL; C itself is allowed   */
+  void* preact;              /* [dev] out: A * B + bias in C's type, or NULL               */
+  int64_t ld_residual;
+  int64_t ld_preact;
+  int32_t bias_dtype;        /* float32, bfloat16 or float16                               */
+  int32_t residual_dtype;    /* float32, bfloat16 or float16                               */
+  int32_t activation;        /* LF_ACT_*                                                   */
+} lf_epilogue;
+
+/* C[r,:] = activation(sum_e data[e] * B[indices[e],:] + bias) + residual[r,:] for the rows
+ * [row_begin, row_end); C, residual and preact start at row row_begin.  Rows without entries get
+ * activation(bias) + residual.  B float32, bfloat16, float16 or e4m3 (b_scale: one float per row of
+ * B, or NULL for any type but e4m3); C float32, bfloat16 or float16.  order (or NULL): entry e takes
+ * data[order[e]] -- A transposed, given by its own indptr and indices, over the values of A.  An
+ * entry whose value is 0 reads nothing of B (nor its scale), so it passes on no NaN or infinity.
+ * nnz: the exact number of entries of the rows.  The workspace holds the sums of rows that several
+ * thread groups share; it may be used again as soon as the call is over on the stream, not by two
+ * calls at a time.  Fewer than 2^31 rows, ldb and ldc below 2^30.  Rows of B off the 16-byte grid are read in
+ * the aligned 16-byte pieces that cover them, as in lf_spmm_csr_f32. */
+size_t lf_spmm_csr_act_workspace_bytes(int64_t nnz, int32_t N, int32_t b_dtype);
+int lf_spmm_csr_act(const int64_t* indptr /*[dev]*/, const int32_t* indices /*[dev]*/,
+                    const float* data /*[dev] or NULL: all ones*/, const int32_t* order /*[dev] or NULL*/,
+                    int64_t row_begin, int64_t row_end, int64_t nnz, const void* B /*[dev]*/, int32_t b_dtype,
+                    int64_t ldb, const float* b_scale /*[dev] or NULL*/, void* C /*[dev]*/, int32_t c_dtype,
+                    int64_t ldc, int32_t N, const lf_epilogue* epilogue /*[host] or NULL*/,
+                    void* workspace /*[dev]*/, size_t workspace_bytes, void* stream);
+
+/* dz = dy * activation'(preact) (in the type of both; NULL: not wanted) and dbias = the sum of its rows
+ * before they are rounded (NULL: not wanted).  preact may be NULL for LF_ACT_NONE. */
+size_t lf_act_backward_workspace_bytes(int64_t rows, int32_t N);
+int lf_act_backward(const void* dy /*[dev]*/, int64_t ld_dy, const void* preact /*[dev]*/, int64_t ld_preact,
+                    int32_t dtype, int32_t activation, void* dz /*[dev] out*/, int64_t ld_dz,
+                    float* dbias /*[dev] out, N*/, int64_t rows, int32_t N, void* workspace /*[dev]*/,
+                    size_t workspace_bytes, void* stream);
+
+/* Gradient of the values: dvalues[e] = <dy[r,:] * activation'(preact[r,:]), B[indices[e],:]> for the
+ * entries e of the rows r of [row_begin, row_end), counted from the first of them; dy and preact start at
+ * row row_begin and have dy_dtype. */
+int lf_spmm_csr_grad_values(const int64_t* indptr /*[dev]*/, const int32_t* indices /*[dev]*/, int64_t row_begin,
+                            int64_t row_end, int64_t nnz, const void* dy /*[dev]*/, int64_t ld_dy,
+                            const void* preact /*[dev]*/, int64_t ld_preact, int32_t dy_dtype, int32_t activation,
+                            const void* B /*[dev]*/, int32_t b_dtype, int64_t ldb, int32_t N,
+                            float* dvalues /*[dev] out*/, void* stream);
+
+/* h = x + residual rounded to `dtype` (the sum is kept in `sum`, which may be x or residual itself; without
+ * a residual h = x and sum is not used), rstd = (mean(h^2) + eps)^(-1/2), y = h * rstd * weight in y_dtype.  For
+ * e4m3 scale[r] = max|y[r,:]| / 448 and y holds y / scale; a row whose largest magnitude is below 448 * 2^-126
+ * is stored as zeros with scale 0, a row with a NaN gets the scale NaN.  rstd: one float per row for the
+ * backward pass, or NULL. */
+int lf_rms_norm(const void* x /*[dev]*/, int32_t dtype, int64_t ld_x, const void* residual /*[dev] or NULL*/,
+                int64_t ld_residual, void* sum /*[dev] out*/, int64_t ld_sum, const void* weight /*[dev] N*/,
+                int32_t weight_dtype, float eps, void* y /*[dev] out*/, int32_t y_dtype, int64_t ld_y,
+                float* scale /*[dev] out, e4m3 only*/, float* rstd /*[dev] out or NULL*/, int64_t rows, int32_t N,
+                void* stream);
+
+/* Gradients of y = h * rstd * weight: dx = rstd * (dy * weight - n * mean(dy * weight * n)) + dsum with
+ * n = h * rstd (dsum: the gradient that reaches h by other ways, or NULL), for x and for the residual alike, in
+ * `dtype` like dy, h and dsum; dweight = sum over the rows of dy * n.  dx may be dy, h or dsum itself. */
+size_t lf_rms_norm_backward_workspace_bytes(int64_t rows, int32_t N);
+int lf_rms_norm_backward(const void* dy /*[dev]*/, int64_t ld_dy, const void* h /*[dev]*/, int64_t ld_h, int32_t dtype,
+                         const void* weight /*[dev] N*/, int32_t weight_dtype, const float* rstd /*[dev]*/,
+                         const void* dsum /*[dev] or NULL*/, int64_t ld_dsum, void* dx /*[dev] out*/, int64_t ld_dx,
+                         float* dweight /*[dev] out, N*/, int64_t rows, int32_t N, void* workspace /*[dev]*/,
+                         size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -31,7 +31,8 @@ LF_OPT_BSR_UMMA_PRODUCER = 9
 LF_OPT_SPMM_GATHER_RING = 10
 LF_OPT_BSR_BLOCK_WARPS = 11
 LF_OPT_SPMM_RING_MIN_SLOTS = 12
-LF_DTYPE_F32, LF_DTYPE_BF16, LF_DTYPE_F16 = 0, 1, 2
+LF_DTYPE_F32, LF_DTYPE_BF16, LF_DTYPE_F16, LF_DTYPE_E4M3 = 0, 1, 2, 3
+LF_ACT_NONE, LF_ACT_RELU, LF_ACT_SILU, LF_ACT_GELU, LF_ACT_GELU_TANH = 0, 1, 2, 3, 4
 LF_SPMM_OVERWRITE = 0
 LF_SPMM_ACCUMULATE = 1
 LF_SPMM_NO_SYNC = 2
@@ -56,6 +57,14 @@ class LfHyb(C.Structure):
         ("part_bucket_off", vp), ("widths", vp), ("ell_rows", vp), ("row_off", vp), ("slot_off", vp),
         ("rows", vp), ("cols", vp), ("vals", vp), ("mask", vp), ("zero_rows", vp),
         ("num_zero_rows", C.c_int64),
+    ]
+
+
+class LfEpilogue(C.Structure):
+    """Mirror of ``struct lf_epilogue``."""
+    _fields_ = [
+        ("bias", vp), ("residual", vp), ("preact", vp), ("ld_residual", C.c_int64), ("ld_preact", C.c_int64),
+        ("bias_dtype", C.c_int32), ("residual_dtype", C.c_int32), ("activation", C.c_int32),
     ]
 
 
@@ -105,6 +114,19 @@ SIGNATURES = {
     "lf_row_stats_blocks": (C.c_int64, [C.c_int64, C.c_int64]),
     "lf_row_stats": (C.c_int, [vp, C.c_int64, C.c_int64, vp, vp]),
     "lf_shard_rows": (C.c_int, [vp, C.c_int64, C.c_int32, vp, vp]),
+    "lf_spmm_csr_act_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int32, C.c_int32]),
+    "lf_spmm_csr_act": (C.c_int, [vp, vp, vp, vp, C.c_int64, C.c_int64, C.c_int64, vp, C.c_int32, C.c_int64, vp, vp, C.c_int32,
+                                  C.c_int64, C.c_int32, C.POINTER(LfEpilogue), vp, C.c_size_t, vp]),
+    "lf_act_backward_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int32]),
+    "lf_act_backward": (C.c_int, [vp, C.c_int64, vp, C.c_int64, C.c_int32, C.c_int32, vp, C.c_int64, vp, C.c_int64, C.c_int32,
+                                  vp, C.c_size_t, vp]),
+    "lf_spmm_csr_grad_values": (C.c_int, [vp, vp, C.c_int64, C.c_int64, C.c_int64, vp, C.c_int64, vp, C.c_int64, C.c_int32,
+                                          C.c_int32, vp, C.c_int32, C.c_int64, C.c_int32, vp, vp]),
+    "lf_rms_norm": (C.c_int, [vp, C.c_int32, C.c_int64, vp, C.c_int64, vp, C.c_int64, vp, C.c_int32, C.c_float, vp, C.c_int32,
+                              C.c_int64, vp, vp, C.c_int64, C.c_int32, vp]),
+    "lf_rms_norm_backward_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int32]),
+    "lf_rms_norm_backward": (C.c_int, [vp, C.c_int64, vp, C.c_int64, C.c_int32, vp, C.c_int32, vp, vp, C.c_int64, vp, C.c_int64,
+                                       vp, C.c_int64, C.c_int32, vp, C.c_size_t, vp]),
 }
 
 _lib: Optional[C.CDLL] = None

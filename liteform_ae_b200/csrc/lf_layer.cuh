@@ -1,0 +1,132 @@
+// Element types, activations and sums shared by the operators of a layer: the CSR product with bias,
+// activation and residual (lf_spmm_act.cu), its gradients (lf_spmm_act_grad.cu) and the root-mean-square norm
+// (lf_rms_norm.cu).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "lf_common.cuh"
+
+namespace lf {
+
+inline bool is_wide_dtype(int32_t dt) { return dt == LF_DTYPE_F32 || dt == LF_DTYPE_BF16 || dt == LF_DTYPE_F16; }
+inline int dtype_bytes(int32_t dt) { return dt == LF_DTYPE_F32 ? 4 : dt == LF_DTYPE_E4M3 ? 1 : 2; }
+inline bool on_grid16(const void* p, int64_t ld, int32_t dt) {   // every row starts on a 16-byte boundary
+  return (uintptr_t)p % 16 == 0 && ld * dtype_bytes(dt) % 16 == 0;
+}
+
+// `Type<LF_DTYPE_...>`: the stored type, and its way to and from float (rounded to nearest, ties to even)
+template <int DT> struct Type;
+template <> struct Type<LF_DTYPE_F32> {
+  using T = float;
+  static __device__ __forceinline__ float get(T v) { return v; }
+  static __device__ __forceinline__ T put(float v) { return v; }
+};
+template <> struct Type<LF_DTYPE_BF16> {
+  using T = __nv_bfloat16;
+  static __device__ __forceinline__ float get(T v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ T put(float v) { return __float2bfloat16_rn(v); }
+};
+template <> struct Type<LF_DTYPE_F16> {
+  using T = __half;
+  static __device__ __forceinline__ float get(T v) { return __half2float(v); }
+  static __device__ __forceinline__ T put(float v) { return __float2half_rn(v); }
+};
+template <> struct Type<LF_DTYPE_E4M3> {   // put: values beyond 448 become 448, NaN stays NaN
+  using T = __nv_fp8_storage_t;
+  static __device__ __forceinline__ float get(T v) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(v, __NV_E4M3))); }
+  static __device__ __forceinline__ T put(float v) { return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
+};
+
+// `n` consecutive elements, from or to an address that is a multiple of their size together (n * bytes <= 16, or
+// a multiple of 16)
+template <int DT, int n>
+struct Pack {
+  static constexpr int kBytes = n * (int)sizeof(typename Type<DT>::T);
+  static constexpr int kWord = kBytes >= 16 ? 16 : kBytes;
+  union {
+    typename Type<DT>::T e[n];
+    uint4 q[(kBytes + 15) / 16];
+    uint2 d;
+    uint32_t w;
+    uint16_t h;
+    uint8_t b;
+  };
+  __device__ __forceinline__ Pack() {}
+  __device__ __forceinline__ void load(const void* p) {
+    if constexpr (kWord == 16) {
+#pragma unroll
+      for (int i = 0; i < kBytes / 16; ++i) q[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    } else if constexpr (kWord == 8) d = __ldg(reinterpret_cast<const uint2*>(p));
+    else if constexpr (kWord == 4) w = __ldg(reinterpret_cast<const uint32_t*>(p));
+    else if constexpr (kWord == 2) h = __ldg(reinterpret_cast<const uint16_t*>(p));
+    else b = __ldg(reinterpret_cast<const uint8_t*>(p));
+  }
+  __device__ __forceinline__ void store(void* p) const {   // written once, read by a later launch: streaming
+    if constexpr (kWord == 16) {
+#pragma unroll
+      for (int i = 0; i < kBytes / 16; ++i) __stcs(reinterpret_cast<uint4*>(p) + i, q[i]);
+    } else if constexpr (kWord == 8) __stcs(reinterpret_cast<uint2*>(p), d);
+    else if constexpr (kWord == 4) __stcs(reinterpret_cast<uint32_t*>(p), w);
+    else if constexpr (kWord == 2) __stcs(reinterpret_cast<uint16_t*>(p), h);
+    else __stcs(reinterpret_cast<uint8_t*>(p), b);
+  }
+  __device__ __forceinline__ float get(int i) const { return Type<DT>::get(e[i]); }
+  __device__ __forceinline__ void put(int i, float v) { e[i] = Type<DT>::put(v); }
+};
+
+// one element of a type that is known at run time only (never 8 bits)
+__device__ __forceinline__ float get_any(const void* p, int64_t i, int dt) {
+  if (dt == LF_DTYPE_F32) return __ldg(reinterpret_cast<const float*>(p) + i);
+  if (dt == LF_DTYPE_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(reinterpret_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ void put_any(void* p, int64_t i, int dt, float v) {
+  if (dt == LF_DTYPE_F32) reinterpret_cast<float*>(p)[i] = v;
+  else if (dt == LF_DTYPE_BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+
+// ---- activations ------------------------------------------------------------------------------------
+// 1 / (1 + exp(-z)); for z so low that the exponential overflows, 0
+__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + expf(-z)); }
+// the tanh form of GELU is z * sigmoid(gelu_arg(z)), since (1 + tanh u) / 2 = sigmoid(2 u)
+__device__ __forceinline__ float gelu_arg(float z) { return 1.5957691216057308f * z * fmaf(0.044715f * z, z, 1.f); }
+
+__device__ __forceinline__ float activate(float z, int act) {
+  switch (act) {
+    case LF_ACT_RELU: return z < 0.f ? 0.f : z;   // a NaN stays one
+    case LF_ACT_SILU: return z * sigmoid(z);
+    case LF_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    case LF_ACT_GELU_TANH: return z * sigmoid(gelu_arg(z));
+    default: return z;
+  }
+}
+
+// beyond +-100 every slope is 0 or 1 to the last bit; so far the formulas stay clear of 0 * infinity
+__device__ __forceinline__ float activate_slope(float z, int act) {
+  z = z > 100.f ? 100.f : z < -100.f ? -100.f : z;
+  switch (act) {
+    case LF_ACT_RELU: return z > 0.f ? 1.f : 0.f;
+    case LF_ACT_SILU: {
+      const float p = sigmoid(z);
+      return p * fmaf(z, 1.f - p, 1.f);
+    }
+    case LF_ACT_GELU: return fmaf(0.5f, erff(z * 0.70710678118654752f), 0.5f) + z * 0.3989422804014327f * expf(-0.5f * z * z);
+    case LF_ACT_GELU_TANH: {
+      const float p = sigmoid(gelu_arg(z));
+      return p * fmaf(z * (1.f - p), 1.5957691216057308f * fmaf(0.134145f * z, z, 1.f), 1.f);
+    }
+    default: return 1.f;
+  }
+}
+
+__device__ __forceinline__ float warp_sum(float v) {   // the same sum in every lane
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+}  // namespace lf

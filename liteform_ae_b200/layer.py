@@ -1,0 +1,366 @@
+"""Operators of a layer around the CSR product: the norm that makes the rows it gathers, the product with
+bias, activation and residual in its epilogue, and the gradients of both.
+
+    n = rms_norm(x, w, residual=r, out_dtype=torch.float8_e4m3fn)       # n.h = x + r, n.y and n.scale its norm
+    y = spmm_csr_act(csr, n.y, scale=n.scale, bias=b, activation="silu", residual=n.h)
+
+and for training, with 16- or 32-bit rows and the transposed pattern that the program keeps beside A:
+
+    z = torch.empty_like(dy);  y = spmm_csr_act(csr, f, bias=b, activation="silu", residual=h, preact=z)
+    g = spmm_csr_act_backward(csr, csr_t, f, dy, preact=z, activation="silu")      # g.dB, g.dvalues, g.dbias
+    dx, dw = rms_norm_backward(g.dB, h, w, n.rstd, dh=dy)                          # dy also reaches h directly
+
+The reference has no counterpart: its product ends with C = A * B (playground_pipline/format_algos.py:1660-1755).
+
+All computation is done by ``liblf_b200.so`` on torch's current stream of the tensors' device; nothing is
+synchronised (except for a ``row_range``, see ``spmm_csr_act``).  The same call on the same inputs gives the same
+bits.  Matrices are dense in their last dimension and may have any row stride of at least their width; a row stride
+and address on 16-byte boundaries is faster.  ``ValueError`` for arguments that do not fit together.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from dataclasses import dataclass
+from typing import NamedTuple, Optional, Tuple
+
+import numpy as np
+
+from . import _cabi
+from ._cabi import LfEpilogue, check, cuda_torch as _torch, on_device, stream_of
+from .hyb import DeviceCsr, Workspace
+
+ACTIVATIONS = {None: _cabi.LF_ACT_NONE, "none": _cabi.LF_ACT_NONE, "relu": _cabi.LF_ACT_RELU, "silu": _cabi.LF_ACT_SILU,
+               "gelu": _cabi.LF_ACT_GELU, "gelu_tanh": _cabi.LF_ACT_GELU_TANH}
+
+_codes = {}
+
+
+def _code(dtype, allowed="wide"):
+    """``LF_DTYPE_*`` of a torch type; ``allowed``: "wide" (16 and 32 bits) or "any" (e4m3 too)."""
+    if not _codes:
+        torch = _torch()
+        _codes.update({torch.float32: _cabi.LF_DTYPE_F32, torch.bfloat16: _cabi.LF_DTYPE_BF16,
+                       torch.float16: _cabi.LF_DTYPE_F16, torch.float8_e4m3fn: _cabi.LF_DTYPE_E4M3})
+    code = _codes.get(dtype)
+    if code is None or (allowed == "wide" and code == _cabi.LF_DTYPE_E4M3):
+        raise ValueError(f"type {dtype} is not supported here")
+    return code
+
+
+def _need(cond, message):
+    if not cond:
+        raise ValueError(message)
+
+
+def _matrix(t, name, rows, N, dev):
+    """Row stride of ``t``, which has to be ``[rows, N]`` on device ``dev`` and dense in a row."""
+    _need(t.dim() == 2 and t.shape[0] == rows and t.shape[1] == N, f"{name} must have shape ({rows}, {N})")
+    _need(t.is_cuda and t.get_device() == dev, f"{name} must be on the device of the other operands")
+    _need(N == 1 or t.stride(1) == 1, f"{name} must be dense in its last dimension")
+    ld = t.stride(0)
+    if rows <= 1:
+        return max(ld, N)
+    _need(ld >= N, f"rows of {name} overlap")
+    return ld
+
+
+def _vector(t, name, n, dev, dtype=None):
+    _need(t.dim() == 1 and t.shape[0] == n and (n <= 1 or t.stride(0) == 1), f"{name} must be a dense vector of {n}")
+    _need(t.is_cuda and t.get_device() == dev, f"{name} must be on the device of the other operands")
+    _need(dtype is None or t.dtype == dtype, f"{name} must be {dtype}")
+    return t.data_ptr()
+
+
+def _scratch(nbytes, workspace, device):
+    if nbytes == 0:
+        return None, 0
+    buf = _torch().empty(nbytes, dtype=_torch().uint8, device=device) if workspace is None else workspace.get(nbytes)
+    return buf, buf.data_ptr()
+
+
+def empty_rows(rows: int, N: int, dtype, device):
+    """``[rows, N]`` uninitialised with every row on a 16-byte boundary (the view of a wider buffer where N does
+    not give that by itself): how the operators allocate 8-bit rows."""
+    torch = _torch()
+    per = 16 // torch.empty(0, dtype=dtype).element_size()
+    wide = -(-N // per) * per
+    t = torch.empty((rows, wide), dtype=dtype, device=device)
+    return t if wide == N else t[:, :N]
+
+
+# ---- norm -------------------------------------------------------------------------------------------
+class NormOutput(NamedTuple):
+    y: "object"                 # normed rows
+    scale: Optional["object"]   # float32, one per row: what e4m3 rows are multiples of (None for other types)
+    h: "object"                 # what was normed: x + residual, or x itself
+    rstd: "object"              # float32, one per row, for the backward pass
+
+
+def rms_norm(x, weight, residual=None, eps: float = 1e-6, out_dtype=None, out=None, scale=None, sum_out=None,
+             rstd=None) -> NormOutput:
+    """``lf_rms_norm``: ``h = x + residual`` in x's type, ``y = h * rstd * weight`` with ``rstd = (mean(h^2) +
+    eps)^(-1/2)``, row by row.  ``out_dtype`` (default: x's): float32, bfloat16, float16, or float8_e4m3fn with one
+    scale per row (``y * scale`` is the row).  ``out``, ``scale``, ``sum_out`` (may be ``x`` or ``residual``) and
+    ``rstd`` take the outputs in place of new tensors."""
+    torch = _torch()
+    _need(x.is_cuda and x.dim() == 2 and x.shape[1] >= 1, "x must be a matrix on a CUDA device")
+    M, N = x.shape
+    dev = x.get_device()
+    code = _code(x.dtype)
+    ld_x = _matrix(x, "x", M, N, dev)
+    w = _vector(weight, "weight", N, dev)
+    w_code = _code(weight.dtype)
+    if out_dtype is None:
+        out_dtype = x.dtype if out is None else out.dtype
+    y_code = _code(out_dtype, "any")
+    e4m3 = y_code == _cabi.LF_DTYPE_E4M3
+    if out is None:
+        out = empty_rows(M, N, out_dtype, x.device) if e4m3 else torch.empty((M, N), dtype=out_dtype, device=x.device)
+    _need(out.dtype == out_dtype, f"out must be {out_dtype}")
+    ld_y = _matrix(out, "out", M, N, dev)
+    h, res_ptr, ld_res, sum_ptr, ld_sum = x, 0, 0, 0, 0
+    if residual is not None:
+        _need(residual.dtype == x.dtype, "the residual must have x's type")
+        res_ptr, ld_res = residual.data_ptr(), _matrix(residual, "residual", M, N, dev)
+        h = torch.empty((M, N), dtype=x.dtype, device=x.device) if sum_out is None else sum_out
+        _need(h.dtype == x.dtype, "sum_out must have x's type")
+        sum_ptr, ld_sum = h.data_ptr(), _matrix(h, "sum_out", M, N, dev)
+    else:
+        _need(sum_out is None, "sum_out goes with a residual")
+    if not e4m3:
+        _need(scale is None, "a scale goes with 8-bit rows")
+    elif scale is None:
+        scale = torch.empty(M, dtype=torch.float32, device=x.device)
+    if rstd is None:
+        rstd = torch.empty(M, dtype=torch.float32, device=x.device)
+    s_ptr = _vector(scale, "scale", M, dev, torch.float32) if e4m3 else 0
+    r_ptr = _vector(rstd, "rstd", M, dev, torch.float32)
+    with on_device(dev):
+        check(_cabi.load().lf_rms_norm(x.data_ptr(), code, ld_x, res_ptr, ld_res, sum_ptr, ld_sum, w, w_code, float(eps),
+                                       out.data_ptr(), y_code, ld_y, s_ptr, r_ptr, M, N, stream_of(dev)))
+    return NormOutput(out, scale, h, rstd)
+
+
+def rms_norm_backward(dy, h, weight, rstd, dh=None, dx=None, dweight=None, workspace: Optional[Workspace] = None):
+    """``lf_rms_norm_backward``: ``(dx, dweight)`` for ``y = h * rstd * weight``; ``dx`` (in dy's type) is the gradient
+    of x and of the residual alike, with ``dh``, the gradient that reaches h by other ways, added; ``dweight`` is
+    float32.  For 8-bit rows pass the gradient of the rows they stand for (the rounding's own is taken as 1).
+    ``dx`` may be ``dy``, ``h`` or ``dh``."""
+    torch = _torch()
+    lib = _cabi.load()
+    _need(dy.is_cuda and dy.dim() == 2 and dy.shape[1] >= 1, "dy must be a matrix on a CUDA device")
+    M, N = dy.shape
+    dev = dy.get_device()
+    code = _code(dy.dtype)
+    _need(h.dtype == dy.dtype and (dh is None or dh.dtype == dy.dtype), "dy, h and dh must have one type")
+    ld_dy, ld_h = _matrix(dy, "dy", M, N, dev), _matrix(h, "h", M, N, dev)
+    ld_dh = 0 if dh is None else _matrix(dh, "dh", M, N, dev)
+    if dx is None:
+        dx = torch.empty((M, N), dtype=dy.dtype, device=dy.device)
+    if dweight is None:
+        dweight = torch.empty(N, dtype=torch.float32, device=dy.device)
+    _need(dx.dtype == dy.dtype, "dx must have dy's type")
+    ld_dx = _matrix(dx, "dx", M, N, dev)
+    w, w_code, r = _vector(weight, "weight", N, dev), _code(weight.dtype), _vector(rstd, "rstd", M, dev, torch.float32)
+    dw = _vector(dweight, "dweight", N, dev, torch.float32)
+    nbytes = lib.lf_rms_norm_backward_workspace_bytes(M, N)
+    with on_device(dev):
+        keep, ws = _scratch(nbytes, workspace, dy.device)
+        check(lib.lf_rms_norm_backward(dy.data_ptr(), ld_dy, h.data_ptr(), ld_h, code, w, w_code, r,
+                                       0 if dh is None else dh.data_ptr(), ld_dh, dx.data_ptr(), ld_dx, dw, M, N, ws, nbytes,
+                                       stream_of(dev)))
+    return dx, dweight
+
+
+# ---- product ----------------------------------------------------------------------------------------
+@dataclass
+class CsrTranspose:
+    """The pattern of a matrix by columns: what the product with A transposed takes beside A's values.
+    ``order[i]`` is the place of entry i among A's entries, so the values are kept once, with A."""
+    indptr: "object"            # torch int64 [K + 1]
+    indices: "object"           # torch int32 [nnz]: rows of A, ascending inside a column
+    order: "object"             # torch int32 [nnz]
+    shape: Tuple[int, int]      # (K, M)
+
+    @property
+    def nnz(self) -> int:
+        return int(self.indices.numel())
+
+    @staticmethod
+    def from_host(indptr, indices, shape, device="cuda") -> "CsrTranspose":
+        """From A's own (host) arrays and shape."""
+        import torch
+        M, K = int(shape[0]), int(shape[1])
+        indptr, indices = np.asarray(indptr, dtype=np.int64), np.asarray(indices)
+        _need(len(indices) < 2 ** 31 and M < 2 ** 31, "at most 2^31 - 1 entries and rows")
+        order = np.argsort(indices, kind="stable")
+        rows = np.repeat(np.arange(M, dtype=np.int32), np.diff(indptr))[order]
+        ptr = np.zeros(K + 1, dtype=np.int64)
+        np.cumsum(np.bincount(indices, minlength=K), out=ptr[1:])
+        up = lambda a: torch.from_numpy(a).to(device)
+        return CsrTranspose(up(ptr), up(rows), up(order.astype(np.int32)), (K, M))
+
+    @staticmethod
+    def of(csr: DeviceCsr) -> "CsrTranspose":
+        """From a matrix in device memory (sorted on the host: done once per matrix)."""
+        return CsrTranspose.from_host(csr.indptr.cpu().numpy(), csr.indices.cpu().numpy(), csr.shape, csr.indptr.device)
+
+
+def _product(lib, a, data, order, r0, r1, nnz, B, b_code, ldb, scale_ptr, out, ldc, N, ep, workspace, dev):
+    nbytes = lib.lf_spmm_csr_act_workspace_bytes(a.nnz, N, b_code)
+    keep, ws = _scratch(nbytes, workspace, B.device)
+    check(lib.lf_spmm_csr_act(a.indptr.data_ptr(), a.indices.data_ptr(), data, order, r0, r1, nnz, B.data_ptr(), b_code, ldb,
+                              scale_ptr, out.data_ptr(), _code(out.dtype), ldc, N, ep, ws, nbytes, stream_of(dev)))
+
+
+def _csr_arrays(a, values, dev):
+    """Addresses of the values and of their order."""
+    transposed = isinstance(a, CsrTranspose)
+    _need(transposed or values is None, "values go with a CsrTranspose; a DeviceCsr has its own")
+    data = values if transposed else a.data
+    for t, name, n in ((a.indptr, "indptr", a.shape[0] + 1), (a.indices, "indices", a.nnz)):
+        _need(t.get_device() == dev and t.is_contiguous() and t.numel() == n, f"{name} must be a dense vector of {n} beside B")
+    if data is None:
+        return 0, 0
+    _need(data.numel() == a.nnz and data.is_contiguous() and data.get_device() == dev and data.dtype == _torch().float32,
+          "the values must be a dense float32 vector, one per entry, beside B")
+    return data.data_ptr(), a.order.data_ptr() if transposed else 0
+
+
+def spmm_csr_act(a, B, scale=None, bias=None, activation: Optional[str] = None, residual=None, out_dtype=None, out=None,
+                 preact=None, row_range=None, values=None, workspace: Optional[Workspace] = None):
+    """``lf_spmm_csr_act``: ``activation(A @ B + bias) + residual`` for a ``DeviceCsr`` (or a ``CsrTranspose`` with A's
+    ``values``, None: all ones).  B: float32, bfloat16, float16, or float8_e4m3fn with ``scale`` (float32, one per row);
+    ``activation``: None, "relu", "silu", "gelu" or "gelu_tanh"; ``out_dtype``: float32, bfloat16 or float16 (default:
+    B's, bfloat16 for 8-bit rows); ``residual`` may be ``out``; ``preact`` (out's type) is filled with ``A @ B + bias`` for
+    the backward pass.  ``row_range=(r0, r1)``: those rows of A only -- their number of entries is read back, which
+    waits for the stream; a ``DeviceCsr`` of a slice of ``indptr`` does not.  Entries are not checked against B's rows:
+    ``DeviceCsr.validate`` does that, once per matrix."""
+    torch = _torch()
+    lib = _cabi.load()
+    _need(B.is_cuda and B.dim() == 2 and B.shape[1] >= 1, "B must be a matrix on a CUDA device")
+    K, N = B.shape
+    dev = B.get_device()
+    _need(K == a.shape[1], "B must have one row per matrix column")
+    b_code = _code(B.dtype, "any")
+    ldb = _matrix(B, "B", K, N, dev)
+    _need(activation in ACTIVATIONS, f"unknown activation {activation!r}")
+    _need(b_code != _cabi.LF_DTYPE_E4M3 or scale is not None, "8-bit rows need their scales")
+    data, order = _csr_arrays(a, values, dev)
+    r0, r1 = (0, a.shape[0]) if row_range is None else (int(row_range[0]), int(row_range[1]))
+    _need(0 <= r0 <= r1 <= a.shape[0], "bad row range")
+    nnz = a.nnz
+    if row_range is not None and (r0, r1) != (0, a.shape[0]):
+        ends = a.indptr[[r0, r1]].cpu()
+        nnz = int(ends[1]) - int(ends[0])
+    if out_dtype is None:
+        out_dtype = out.dtype if out is not None else torch.bfloat16 if b_code == _cabi.LF_DTYPE_E4M3 else B.dtype
+    if out is None:
+        out = torch.empty((r1 - r0, N), dtype=out_dtype, device=B.device)
+    _need(out.dtype == out_dtype, f"out must be {out_dtype}")
+    ldc = _matrix(out, "out", r1 - r0, N, dev)
+    ep = LfEpilogue()
+    ep.activation = ACTIVATIONS[activation]
+    if bias is not None:
+        ep.bias, ep.bias_dtype = _vector(bias, "bias", N, dev), _code(bias.dtype)
+    if residual is not None:
+        ep.ld_residual = _matrix(residual, "residual", r1 - r0, N, dev)
+        ep.residual, ep.residual_dtype = residual.data_ptr(), _code(residual.dtype)
+        _need(residual.data_ptr() != out.data_ptr() or (residual.dtype == out_dtype and ep.ld_residual == ldc),
+              "a residual at out's address must be out")
+    if preact is not None:
+        _need(preact.dtype == out_dtype, f"preact must be {out_dtype}")
+        ep.preact, ep.ld_preact = preact.data_ptr(), _matrix(preact, "preact", r1 - r0, N, dev)
+    s_ptr = 0 if scale is None else _vector(scale, "scale", K, dev, torch.float32)
+    with on_device(dev):
+        _product(lib, a, data, order, r0, r1, nnz, B, b_code, ldb, s_ptr, out, ldc, N, C.byref(ep), workspace, dev)
+    return out
+
+
+def act_backward(dy, preact=None, activation: Optional[str] = None, dz=None, need_dz: bool = True, need_dbias: bool = True,
+                 dbias=None, workspace: Optional[Workspace] = None):
+    """``lf_act_backward``: ``(dz, dbias)`` with ``dz = dy * activation'(preact)`` in dy's type and ``dbias`` the float32
+    sum of its rows before they are rounded; what is not needed is None."""
+    torch = _torch()
+    lib = _cabi.load()
+    _need(dy.is_cuda and dy.dim() == 2 and dy.shape[1] >= 1, "dy must be a matrix on a CUDA device")
+    _need(activation in ACTIVATIONS, f"unknown activation {activation!r}")
+    act = ACTIVATIONS[activation]
+    M, N = dy.shape
+    dev = dy.get_device()
+    code, ld_dy, ld_z = _code(dy.dtype), _matrix(dy, "dy", M, N, dev), 0
+    if act != _cabi.LF_ACT_NONE:
+        _need(preact is not None and preact.dtype == dy.dtype, "preact must be given, in dy's type")
+        ld_z = _matrix(preact, "preact", M, N, dev)
+    if dz is None and need_dz:
+        dz = torch.empty((M, N), dtype=dy.dtype, device=dy.device)
+    if dbias is None and need_dbias:
+        dbias = torch.empty(N, dtype=torch.float32, device=dy.device)
+    _need(dz is not None or dbias is not None, "nothing to compute")
+    _need(dz is None or dz.dtype == dy.dtype, "dz must have dy's type")
+    ld_dz = 0 if dz is None else _matrix(dz, "dz", M, N, dev)
+    b_ptr = 0 if dbias is None else _vector(dbias, "dbias", N, dev, torch.float32)
+    nbytes = 0 if dbias is None else lib.lf_act_backward_workspace_bytes(M, N)
+    with on_device(dev):
+        keep, ws = _scratch(nbytes, workspace, dy.device)
+        check(lib.lf_act_backward(dy.data_ptr(), ld_dy, 0 if act == _cabi.LF_ACT_NONE else preact.data_ptr(), ld_z, code, act,
+                                  0 if dz is None else dz.data_ptr(), ld_dz, b_ptr, M, N, ws, nbytes, stream_of(dev)))
+    return dz, dbias
+
+
+def spmm_csr_grad_values(a: DeviceCsr, B, dy, preact=None, activation: Optional[str] = None, out=None):
+    """``lf_spmm_csr_grad_values``: the gradient of A's values, ``dvalues[e] = <dz[row of e], B[column of e]>`` with
+    ``dz = dy * activation'(preact)`` not rounded in between; float32, one per entry."""
+    torch = _torch()
+    _need(B.is_cuda and B.dim() == 2 and B.shape[1] >= 1, "B must be a matrix on a CUDA device")
+    K, N = B.shape
+    M, dev = a.shape[0], B.get_device()
+    _need(K == a.shape[1], "B must have one row per matrix column")
+    _need(activation in ACTIVATIONS, f"unknown activation {activation!r}")
+    act = ACTIVATIONS[activation]
+    _csr_arrays(a, None, dev)
+    ldb, ld_dy, ld_z = _matrix(B, "B", K, N, dev), _matrix(dy, "dy", M, N, dev), 0
+    if act != _cabi.LF_ACT_NONE:
+        _need(preact is not None and preact.dtype == dy.dtype, "preact must be given, in dy's type")
+        ld_z = _matrix(preact, "preact", M, N, dev)
+    if out is None:
+        out = torch.empty(a.nnz, dtype=torch.float32, device=B.device)
+    o_ptr = _vector(out, "out", a.nnz, dev, torch.float32)
+    with on_device(dev):
+        check(_cabi.load().lf_spmm_csr_grad_values(
+            a.indptr.data_ptr(), a.indices.data_ptr(), 0, M, a.nnz, dy.data_ptr(), ld_dy,
+            0 if act == _cabi.LF_ACT_NONE else preact.data_ptr(), ld_z, _code(dy.dtype), act, B.data_ptr(), _code(B.dtype), ldb,
+            N, o_ptr, stream_of(dev)))
+    return out
+
+
+class ActGradients(NamedTuple):
+    dB: Optional["object"]        # in B's type
+    dvalues: Optional["object"]   # float32, one per entry of A
+    dbias: Optional["object"]     # float32
+
+
+def spmm_csr_act_backward(a: DeviceCsr, a_t: Optional[CsrTranspose], B, dy, preact=None, activation: Optional[str] = None,
+                          need=("dB", "dvalues", "dbias"), workspace: Optional[Workspace] = None) -> ActGradients:
+    """Gradients of ``spmm_csr_act(a, B, bias=..., activation=..., preact=...)`` from ``dy``, the gradient of its result
+    (which is also that of the residual): ``act_backward``, ``A^T @ dz`` and ``spmm_csr_grad_values``.  ``preact`` and dy
+    have one type, 16 or 32 bits like B (8-bit rows have no gradient here); ``need`` names the ones wanted, ``a_t`` is
+    used for dB only.  dz is rounded to dy's type for dB; dvalues and dbias take it unrounded."""
+    unknown = set(need) - {"dB", "dvalues", "dbias"}
+    _need(not unknown, f"unknown gradient {sorted(unknown)}")
+    _need(activation in ACTIVATIONS, f"unknown activation {activation!r}")
+    _code(B.dtype)
+    dB = dvalues = dbias = None
+    dz = dy
+    plain = ACTIVATIONS[activation] == _cabi.LF_ACT_NONE
+    _need("dB" not in need or (a_t is not None and a_t.shape == (a.shape[1], a.shape[0]) and a_t.nnz == a.nnz),
+          "dB needs the transposed pattern of a")
+    want_dz = "dB" in need and not plain
+    if want_dz or "dbias" in need:
+        got, dbias = act_backward(dy, preact, activation, need_dz=want_dz, need_dbias="dbias" in need, workspace=workspace)
+        dz = got if want_dz else dy
+    if "dB" in need:
+        dB = spmm_csr_act(a_t, dz, values=a.data, out_dtype=B.dtype, workspace=workspace)
+    if "dvalues" in need:
+        dvalues = spmm_csr_grad_values(a, B, dy, preact, activation)
+    return ActGradients(dB, dvalues, dbias)

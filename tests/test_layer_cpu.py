@@ -1,0 +1,137 @@
+"""Refusals of the layer operators that need no GPU, the transposed pattern, and the test's own plain forms."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import layer_reference as ref
+from liteform_ae_b200 import _cabi, layer
+
+BAD, SMALL = _cabi.LF_ERR_INVALID_ARGUMENT, _cabi.LF_ERR_WORKSPACE_TOO_SMALL
+P = 4096    # stands for a device address: refused calls read nothing
+F32, BF16, E4M3 = _cabi.LF_DTYPE_F32, _cabi.LF_DTYPE_BF16, _cabi.LF_DTYPE_E4M3
+
+
+def norm(**kw):
+    a = dict(x=P, dtype=F32, ld_x=8, res=0, ld_res=0, sum=0, ld_sum=0, w=P, wd=F32, eps=1e-6, y=P, yd=F32, ld_y=8, scale=0,
+             rstd=0, rows=2, N=8)
+    a.update(kw)
+    return _cabi.load().lf_rms_norm(*a.values(), 0)
+
+
+@pytest.mark.parametrize("kw", [dict(N=0), dict(rows=-1), dict(ld_x=7), dict(ld_y=7), dict(dtype=E4M3), dict(dtype=7),
+                                dict(wd=E4M3), dict(yd=4), dict(eps=-1.0), dict(eps=float("nan")), dict(x=0), dict(w=0),
+                                dict(y=0), dict(res=P, ld_res=8), dict(res=P, ld_res=7, sum=P, ld_sum=8),
+                                dict(res=P, ld_res=8, sum=P, ld_sum=7), dict(yd=E4M3)])
+def test_norm_refusals(kw):
+    assert norm(**kw) == BAD and _cabi.load().lf_last_error()
+
+
+def test_norm_of_no_rows_does_nothing():
+    assert norm(rows=0, x=0, w=0, y=0) == 0
+
+
+def norm_grad(**kw):
+    a = dict(dy=P, ld_dy=8, h=P, ld_h=8, dtype=F32, w=P, wd=F32, rstd=P, ds=0, ld_ds=0, dx=P, ld_dx=8, dw=P, rows=2, N=8, ws=P,
+             nws=1 << 20)
+    a.update(kw)
+    return _cabi.load().lf_rms_norm_backward(*a.values(), 0)
+
+
+@pytest.mark.parametrize("kw", [dict(N=0), dict(rows=-1), dict(ld_dy=7), dict(ld_h=7), dict(ld_dx=7), dict(ds=P, ld_ds=7),
+                                dict(dtype=E4M3), dict(wd=9), dict(dy=0), dict(h=0), dict(w=0), dict(rstd=0), dict(dx=0), dict(dw=0)])
+def test_norm_backward_refusals(kw):
+    assert norm_grad(**kw) == BAD
+
+
+@pytest.mark.parametrize("kw", [dict(nws=0), dict(ws=0), dict(nws=63)])
+def test_norm_backward_workspace(kw):
+    assert norm_grad(**kw) == SMALL
+
+
+def product(ep=None, **kw):
+    a = dict(indptr=P, indices=P, data=P, order=0, r0=0, r1=2, nnz=4, B=P, bd=F32, ldb=8, scale=0, C=P, cd=F32, ldc=8, N=8,
+             ep=None if ep is None else C.byref(_cabi.LfEpilogue(**ep)), ws=P, nws=1 << 30)
+    a.update(kw)
+    return _cabi.load().lf_spmm_csr_act(*a.values(), 0)
+
+
+@pytest.mark.parametrize("kw", [dict(N=0), dict(ldb=7), dict(ldc=7), dict(ldb=1 << 30), dict(ldc=1 << 30), dict(r0=-1), dict(r0=3),
+                                dict(r1=1 << 31), dict(nnz=-1), dict(bd=4), dict(cd=E4M3), dict(bd=E4M3), dict(indptr=0),
+                                dict(C=0), dict(indices=0), dict(B=0), dict(order=P, data=0), dict(order=P, nnz=1 << 31),
+                                dict(ep=dict(activation=5)), dict(ep=dict(activation=-1)), dict(ep=dict(bias=P, bias_dtype=E4M3)),
+                                dict(ep=dict(residual=P, residual_dtype=E4M3, ld_residual=8)),
+                                dict(ep=dict(residual=P, residual_dtype=F32, ld_residual=7)),
+                                dict(ep=dict(preact=P, ld_preact=7))])
+def test_product_refusals(kw):
+    assert product(**kw) == BAD
+
+
+def test_product_of_no_rows_does_nothing():
+    assert product(r1=0, indptr=0, C=0) == 0
+
+
+def act_grad(**kw):
+    a = dict(dy=P, ld_dy=8, z=P, ld_z=8, dtype=F32, act=_cabi.LF_ACT_SILU, dz=P, ld_dz=8, db=P, rows=2, N=8, ws=P, nws=1 << 20)
+    a.update(kw)
+    return _cabi.load().lf_act_backward(*a.values(), 0)
+
+
+@pytest.mark.parametrize("kw", [dict(N=0), dict(rows=-1), dict(dtype=E4M3), dict(act=9), dict(dz=0, db=0), dict(dy=0), dict(z=0),
+                                dict(ld_dy=7), dict(ld_z=7), dict(ld_dz=7)])
+def test_act_backward_refusals(kw):
+    assert act_grad(**kw) == BAD
+
+
+def test_act_backward_workspace():
+    assert act_grad(nws=0) == SMALL and act_grad(ws=0) == SMALL
+
+
+def value_grad(**kw):
+    a = dict(indptr=P, indices=P, r0=0, r1=2, nnz=4, dy=P, ld_dy=8, z=P, ld_z=8, dyd=F32, act=_cabi.LF_ACT_SILU, B=P, bd=F32, ldb=8,
+             N=8, dv=P)
+    a.update(kw)
+    return _cabi.load().lf_spmm_csr_grad_values(*a.values(), 0)
+
+
+@pytest.mark.parametrize("kw", [dict(N=0), dict(ldb=7), dict(ldb=1 << 30), dict(ld_dy=7), dict(r0=3), dict(r0=-1), dict(nnz=-1),
+                                dict(bd=E4M3), dict(dyd=E4M3), dict(act=9), dict(indptr=0), dict(indices=0), dict(dy=0), dict(B=0),
+                                dict(dv=0), dict(z=0), dict(ld_z=7)])
+def test_value_grad_refusals(kw):
+    assert value_grad(**kw) == BAD
+
+
+def test_epilogue_struct_layout():
+    assert C.sizeof(_cabi.LfEpilogue) == 3 * 8 + 2 * 8 + 3 * 4 + 4
+
+
+def test_workspace_queries_are_pure():
+    lib = _cabi.load()
+    assert lib.lf_rms_norm_backward_workspace_bytes(0, 8) == 0
+    assert lib.lf_rms_norm_backward_workspace_bytes(1000, 8) >= 32
+    assert lib.lf_act_backward_workspace_bytes(1000, 8) >= 32
+    sizes = [lib.lf_spmm_csr_act_workspace_bytes(n, 64, BF16) for n in (0, 1, 1000, 10 ** 6, 10 ** 8)]
+    assert sizes == sorted(sizes)
+
+
+@pytest.mark.parametrize("shape,seed", [((0, 5), 0), ((5, 0), 0), ((1, 1), 1), ((7, 12), 2), ((60, 31), 3)])
+def test_transposed_pattern(shape, seed):
+    import scipy.sparse as sp
+    rng = np.random.default_rng(seed)
+    m = sp.csr_matrix((rng.random(shape) < 0.2).astype(np.float32) * rng.random(shape).astype(np.float32))
+    m.sort_indices()
+    t = layer.CsrTranspose.from_host(m.indptr, m.indices, m.shape, "cpu")
+    want = m.T.tocsr()
+    want.sort_indices()
+    assert t.shape == m.shape[::-1] and t.nnz == m.nnz
+    assert np.array_equal(t.indptr.numpy(), want.indptr) and np.array_equal(t.indices.numpy(), want.indices)
+    assert np.array_equal(m.data[t.order.numpy()], want.data)
+
+
+@pytest.mark.parametrize("name", ref.ACTS)
+def test_slopes_by_differences(name):
+    z = torch.linspace(-9, 9, 1801, dtype=torch.float64) + 1e-3     # clear of the kink
+    d = 1e-5
+    diff = (ref.act(z + d, name) - ref.act(z - d, name)) / (2 * d)
+    assert float((diff - ref.slope(z, name)).abs().max()) < 1e-8
