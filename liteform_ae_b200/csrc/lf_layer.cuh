@@ -64,6 +64,24 @@ struct Pack {
     else if constexpr (kWord == 2) h = __ldg(reinterpret_cast<const uint16_t*>(p));
     else b = __ldg(reinterpret_cast<const uint8_t*>(p));
   }
+  __device__ __forceinline__ void fetch(const void* p) {   // read once, by the thread that may write there later: streaming
+    if constexpr (kWord == 16) {
+#pragma unroll
+      for (int i = 0; i < kBytes / 16; ++i) q[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+    } else if constexpr (kWord == 8) d = __ldcs(reinterpret_cast<const uint2*>(p));
+    else if constexpr (kWord == 4) w = __ldcs(reinterpret_cast<const uint32_t*>(p));
+    else if constexpr (kWord == 2) h = __ldcs(reinterpret_cast<const uint16_t*>(p));
+    else b = __ldcs(reinterpret_cast<const uint8_t*>(p));
+  }
+  __device__ __forceinline__ void keep(void* p) const {   // what the next launch gathers stays in the L2 if it can
+    if constexpr (kWord == 16) {
+#pragma unroll
+      for (int i = 0; i < kBytes / 16; ++i) reinterpret_cast<uint4*>(p)[i] = q[i];
+    } else if constexpr (kWord == 8) *reinterpret_cast<uint2*>(p) = d;
+    else if constexpr (kWord == 4) *reinterpret_cast<uint32_t*>(p) = w;
+    else if constexpr (kWord == 2) *reinterpret_cast<uint16_t*>(p) = h;
+    else *reinterpret_cast<uint8_t*>(p) = b;
+  }
   __device__ __forceinline__ void store(void* p) const {   // written once, read by a later launch: streaming
     if constexpr (kWord == 16) {
 #pragma unroll
@@ -74,7 +92,19 @@ struct Pack {
     else __stcs(reinterpret_cast<uint8_t*>(p), b);
   }
   __device__ __forceinline__ float get(int i) const { return Type<DT>::get(e[i]); }
-  __device__ __forceinline__ void put(int i, float v) { e[i] = Type<DT>::put(v); }
+  __device__ __forceinline__ void put(const float* v) {   // two at a time where the type has such a conversion
+    if constexpr (n % 2 == 0 && DT != LF_DTYPE_F32) {
+#pragma unroll
+      for (int i = 0; i < n; i += 2) {
+        if constexpr (DT == LF_DTYPE_BF16) *reinterpret_cast<__nv_bfloat162*>(e + i) = __floats2bfloat162_rn(v[i], v[i + 1]);
+        else if constexpr (DT == LF_DTYPE_F16) *reinterpret_cast<__half2*>(e + i) = __floats2half2_rn(v[i], v[i + 1]);
+        else *reinterpret_cast<__nv_fp8x2_storage_t*>(e + i) = __nv_cvt_float2_to_fp8x2(make_float2(v[i], v[i + 1]), __NV_SATFINITE, __NV_E4M3);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < n; ++i) e[i] = Type<DT>::put(v[i]);
+    }
+  }
 };
 
 // one element of a type that is known at run time only (never 8 bits)

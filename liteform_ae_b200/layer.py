@@ -54,21 +54,42 @@ def _need(cond, message):
 
 def _matrix(t, name, rows, N, dev):
     """Row stride of ``t``, which has to be ``[rows, N]`` on device ``dev`` and dense in a row."""
-    _need(t.dim() == 2 and t.shape[0] == rows and t.shape[1] == N, f"{name} must have shape ({rows}, {N})")
-    _need(t.is_cuda and t.get_device() == dev, f"{name} must be on the device of the other operands")
-    _need(N == 1 or t.stride(1) == 1, f"{name} must be dense in its last dimension")
-    ld = t.stride(0)
-    if rows <= 1:
-        return max(ld, N)
-    _need(ld >= N, f"rows of {name} overlap")
+    if t.shape != (rows, N):
+        raise ValueError(f"{name} must have shape ({rows}, {N})")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} must be on the device of the other operands")
+    ld, inner = t.stride()
+    if inner != 1 and N != 1:
+        raise ValueError(f"{name} must be dense in its last dimension")
+    if ld < N:
+        if rows > 1:
+            raise ValueError(f"rows of {name} overlap")
+        return N
     return ld
 
 
 def _vector(t, name, n, dev, dtype=None):
-    _need(t.dim() == 1 and t.shape[0] == n and (n <= 1 or t.stride(0) == 1), f"{name} must be a dense vector of {n}")
-    _need(t.is_cuda and t.get_device() == dev, f"{name} must be on the device of the other operands")
-    _need(dtype is None or t.dtype == dtype, f"{name} must be {dtype}")
+    if t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name} must be a dense vector of {n}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} must be on the device of the other operands")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}")
     return t.data_ptr()
+
+
+def _first(t, name):
+    """``(rows, N, device)`` of the operand that the others have to fit."""
+    if not t.is_cuda or t.dim() != 2 or t.shape[1] < 1:
+        raise ValueError(f"{name} must be a matrix on a CUDA device")
+    return t.shape[0], t.shape[1], t.get_device()
+
+
+def _act_code(activation):
+    code = ACTIVATIONS.get(activation)
+    if code is None:
+        raise ValueError(f"unknown activation {activation!r}")
+    return code
 
 
 def _scratch(nbytes, workspace, device):
@@ -82,7 +103,7 @@ def empty_rows(rows: int, N: int, dtype, device):
     """``[rows, N]`` uninitialised with every row on a 16-byte boundary (the view of a wider buffer where N does
     not give that by itself): how the operators allocate 8-bit rows."""
     torch = _torch()
-    per = 16 // torch.empty(0, dtype=dtype).element_size()
+    per = 16 // dtype.itemsize
     wide = -(-N // per) * per
     t = torch.empty((rows, wide), dtype=dtype, device=device)
     return t if wide == N else t[:, :N]
@@ -103,9 +124,7 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, out_dtype=None, out=No
     scale per row (``y * scale`` is the row).  ``out``, ``scale``, ``sum_out`` (may be ``x`` or ``residual``) and
     ``rstd`` take the outputs in place of new tensors."""
     torch = _torch()
-    _need(x.is_cuda and x.dim() == 2 and x.shape[1] >= 1, "x must be a matrix on a CUDA device")
-    M, N = x.shape
-    dev = x.get_device()
+    M, N, dev = _first(x, "x")
     code = _code(x.dtype)
     ld_x = _matrix(x, "x", M, N, dev)
     w = _vector(weight, "weight", N, dev)
@@ -116,7 +135,7 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, out_dtype=None, out=No
     e4m3 = y_code == _cabi.LF_DTYPE_E4M3
     if out is None:
         out = empty_rows(M, N, out_dtype, x.device) if e4m3 else torch.empty((M, N), dtype=out_dtype, device=x.device)
-    _need(out.dtype == out_dtype, f"out must be {out_dtype}")
+    _need(out.dtype == out_dtype, "out must have out_dtype")
     ld_y = _matrix(out, "out", M, N, dev)
     h, res_ptr, ld_res, sum_ptr, ld_sum = x, 0, 0, 0, 0
     if residual is not None:
@@ -148,9 +167,7 @@ def rms_norm_backward(dy, h, weight, rstd, dh=None, dx=None, dweight=None, works
     ``dx`` may be ``dy``, ``h`` or ``dh``."""
     torch = _torch()
     lib = _cabi.load()
-    _need(dy.is_cuda and dy.dim() == 2 and dy.shape[1] >= 1, "dy must be a matrix on a CUDA device")
-    M, N = dy.shape
-    dev = dy.get_device()
+    M, N, dev = _first(dy, "dy")
     code = _code(dy.dtype)
     _need(h.dtype == dy.dtype and (dh is None or dh.dtype == dy.dtype), "dy, h and dh must have one type")
     ld_dy, ld_h = _matrix(dy, "dy", M, N, dev), _matrix(h, "h", M, N, dev)
@@ -218,8 +235,9 @@ def _csr_arrays(a, values, dev):
     transposed = isinstance(a, CsrTranspose)
     _need(transposed or values is None, "values go with a CsrTranspose; a DeviceCsr has its own")
     data = values if transposed else a.data
-    for t, name, n in ((a.indptr, "indptr", a.shape[0] + 1), (a.indices, "indices", a.nnz)):
-        _need(t.get_device() == dev and t.is_contiguous() and t.numel() == n, f"{name} must be a dense vector of {n} beside B")
+    _need(a.indptr.get_device() == dev and a.indptr.is_contiguous() and a.indptr.numel() == a.shape[0] + 1,
+          "indptr must be a dense vector of one more than the rows, beside B")
+    _need(a.indices.get_device() == dev and a.indices.is_contiguous(), "indices must be a dense vector beside B")
     if data is None:
         return 0, 0
     _need(data.numel() == a.nnz and data.is_contiguous() and data.get_device() == dev and data.dtype == _torch().float32,
@@ -238,13 +256,11 @@ def spmm_csr_act(a, B, scale=None, bias=None, activation: Optional[str] = None, 
     ``DeviceCsr.validate`` does that, once per matrix."""
     torch = _torch()
     lib = _cabi.load()
-    _need(B.is_cuda and B.dim() == 2 and B.shape[1] >= 1, "B must be a matrix on a CUDA device")
-    K, N = B.shape
-    dev = B.get_device()
+    K, N, dev = _first(B, "B")
     _need(K == a.shape[1], "B must have one row per matrix column")
     b_code = _code(B.dtype, "any")
     ldb = _matrix(B, "B", K, N, dev)
-    _need(activation in ACTIVATIONS, f"unknown activation {activation!r}")
+    act = _act_code(activation)
     _need(b_code != _cabi.LF_DTYPE_E4M3 or scale is not None, "8-bit rows need their scales")
     data, order = _csr_arrays(a, values, dev)
     r0, r1 = (0, a.shape[0]) if row_range is None else (int(row_range[0]), int(row_range[1]))
@@ -257,10 +273,10 @@ def spmm_csr_act(a, B, scale=None, bias=None, activation: Optional[str] = None, 
         out_dtype = out.dtype if out is not None else torch.bfloat16 if b_code == _cabi.LF_DTYPE_E4M3 else B.dtype
     if out is None:
         out = torch.empty((r1 - r0, N), dtype=out_dtype, device=B.device)
-    _need(out.dtype == out_dtype, f"out must be {out_dtype}")
+    _need(out.dtype == out_dtype, "out must have out_dtype")
     ldc = _matrix(out, "out", r1 - r0, N, dev)
     ep = LfEpilogue()
-    ep.activation = ACTIVATIONS[activation]
+    ep.activation = act
     if bias is not None:
         ep.bias, ep.bias_dtype = _vector(bias, "bias", N, dev), _code(bias.dtype)
     if residual is not None:
@@ -269,7 +285,7 @@ def spmm_csr_act(a, B, scale=None, bias=None, activation: Optional[str] = None, 
         _need(residual.data_ptr() != out.data_ptr() or (residual.dtype == out_dtype and ep.ld_residual == ldc),
               "a residual at out's address must be out")
     if preact is not None:
-        _need(preact.dtype == out_dtype, f"preact must be {out_dtype}")
+        _need(preact.dtype == out_dtype, "preact must have the result's type")
         ep.preact, ep.ld_preact = preact.data_ptr(), _matrix(preact, "preact", r1 - r0, N, dev)
     s_ptr = 0 if scale is None else _vector(scale, "scale", K, dev, torch.float32)
     with on_device(dev):
@@ -283,11 +299,8 @@ def act_backward(dy, preact=None, activation: Optional[str] = None, dz=None, nee
     sum of its rows before they are rounded; what is not needed is None."""
     torch = _torch()
     lib = _cabi.load()
-    _need(dy.is_cuda and dy.dim() == 2 and dy.shape[1] >= 1, "dy must be a matrix on a CUDA device")
-    _need(activation in ACTIVATIONS, f"unknown activation {activation!r}")
-    act = ACTIVATIONS[activation]
-    M, N = dy.shape
-    dev = dy.get_device()
+    M, N, dev = _first(dy, "dy")
+    act = _act_code(activation)
     code, ld_dy, ld_z = _code(dy.dtype), _matrix(dy, "dy", M, N, dev), 0
     if act != _cabi.LF_ACT_NONE:
         _need(preact is not None and preact.dtype == dy.dtype, "preact must be given, in dy's type")
@@ -312,12 +325,10 @@ def spmm_csr_grad_values(a: DeviceCsr, B, dy, preact=None, activation: Optional[
     """``lf_spmm_csr_grad_values``: the gradient of A's values, ``dvalues[e] = <dz[row of e], B[column of e]>`` with
     ``dz = dy * activation'(preact)`` not rounded in between; float32, one per entry."""
     torch = _torch()
-    _need(B.is_cuda and B.dim() == 2 and B.shape[1] >= 1, "B must be a matrix on a CUDA device")
-    K, N = B.shape
-    M, dev = a.shape[0], B.get_device()
+    K, N, dev = _first(B, "B")
+    M = a.shape[0]
     _need(K == a.shape[1], "B must have one row per matrix column")
-    _need(activation in ACTIVATIONS, f"unknown activation {activation!r}")
-    act = ACTIVATIONS[activation]
+    act = _act_code(activation)
     _csr_arrays(a, None, dev)
     ldb, ld_dy, ld_z = _matrix(B, "B", K, N, dev), _matrix(dy, "dy", M, N, dev), 0
     if act != _cabi.LF_ACT_NONE:
@@ -347,12 +358,11 @@ def spmm_csr_act_backward(a: DeviceCsr, a_t: Optional[CsrTranspose], B, dy, prea
     have one type, 16 or 32 bits like B (8-bit rows have no gradient here); ``need`` names the ones wanted, ``a_t`` is
     used for dB only.  dz is rounded to dy's type for dB; dvalues and dbias take it unrounded."""
     unknown = set(need) - {"dB", "dvalues", "dbias"}
-    _need(not unknown, f"unknown gradient {sorted(unknown)}")
-    _need(activation in ACTIVATIONS, f"unknown activation {activation!r}")
+    _need(not unknown, "need names dB, dvalues and dbias")
     _code(B.dtype)
     dB = dvalues = dbias = None
     dz = dy
-    plain = ACTIVATIONS[activation] == _cabi.LF_ACT_NONE
+    plain = _act_code(activation) == _cabi.LF_ACT_NONE
     _need("dB" not in need or (a_t is not None and a_t.shape == (a.shape[1], a.shape[0]) and a_t.nnz == a.nnz),
           "dB needs the transposed pattern of a")
     want_dz = "dB" in need and not plain
