@@ -12,7 +12,7 @@
 namespace lf {
 
 inline bool is_wide_dtype(int32_t dt) { return dt == LF_DTYPE_F32 || dt == LF_DTYPE_BF16 || dt == LF_DTYPE_F16; }
-inline int dtype_bytes(int32_t dt) { return dt == LF_DTYPE_F32 ? 4 : dt == LF_DTYPE_E4M3 ? 1 : 2; }
+__host__ __device__ inline int dtype_bytes(int32_t dt) { return dt == LF_DTYPE_F32 ? 4 : dt == LF_DTYPE_E4M3 ? 1 : 2; }
 inline bool on_grid16(const void* p, int64_t ld, int32_t dt) {   // every row starts on a 16-byte boundary
   return (uintptr_t)p % 16 == 0 && ld * dtype_bytes(dt) % 16 == 0;
 }
@@ -119,15 +119,22 @@ __device__ __forceinline__ void put_any(void* p, int64_t i, int dt, float v) {
   else reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // ---- activations ------------------------------------------------------------------------------------
 // 1 / (1 + exp(-z)); for z so low that the exponential overflows, 0
 __device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + expf(-z)); }
 // the tanh form of GELU is z * sigmoid(gelu_arg(z)), since (1 + tanh u) / 2 = sigmoid(2 u)
-__device__ __forceinline__ float gelu_arg(float z) { return 1.5957691216057308f * z * fmaf(0.044715f * z, z, 1.f); }
+constexpr float kGelu0 = 1.5957691216057308f, kGelu1 = 0.044715f;
+__device__ __forceinline__ float gelu_arg(float z) { return z * fmaf(kGelu0 * kGelu1 * z, z, kGelu0); }
 
 __device__ __forceinline__ float activate(float z, int act) {
   switch (act) {
-    case LF_ACT_RELU: return z < 0.f ? 0.f : z;   // a NaN stays one
+    case LF_ACT_RELU: return max_nan(z, 0.f);
     case LF_ACT_SILU: return z * sigmoid(z);
     case LF_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
     case LF_ACT_GELU_TANH: return z * sigmoid(gelu_arg(z));

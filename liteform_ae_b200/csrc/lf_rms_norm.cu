@@ -19,12 +19,6 @@ struct NormArgs {
   float eps;
 };
 
-__device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either is
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // value and sum over a block of 256 threads; every thread gets it
 __device__ __forceinline__ float block_sum(float v, float* smem) {
   v = warp_sum(v);

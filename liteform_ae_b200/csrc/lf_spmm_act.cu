@@ -1,57 +1,371 @@
 // CSR product with the end of a layer in its epilogue: Y = act(A * B + bias) + residual.
-#include "lf_layer.cuh"
+//
+// Two launches.  In the first a warp takes a range of entries and does the rows in it (lf_layer_rows.cuh); a group of
+// lanes that has summed up its row runs the epilogue on its registers, the residual having been fetched along with the rows
+// of B.  The second launch adds up, in order, the pieces of rows that several ranges share, and does the rows without
+// entries.
+#include <type_traits>
+
+#include "lf_layer_rows.cuh"
 
 namespace lf {
 namespace {
 
 struct ActArgs {
-  const int64_t* indptr;
+  const int64_t* indptr;   // of row_begin
   const int32_t* indices;
   const float* data;       // or NULL: all ones
   const int32_t* order;    // data of entry e is data[order[e]], or NULL: data[e]
-  int64_t row_begin, rows, nnz;
+  int64_t nnz;
   const void* B;
   const float* b_scale;    // or NULL
-  int64_t ldb;
   const void* bias;
   const void* residual;
   void* preact;
   void* C;
-  int64_t ld_res, ld_pre, ldc;
-  int N, bias_dtype, res_dtype, c_dtype, act;
+  float* partial;          // [2 * ranges][ld_partial]: sums of a range's first row, where it started earlier, and
+  int64_t ld_partial;      //   of its last row, where it goes on
+  uint32_t pitch_b, pitch_res, pitch_pre, pitch_c;   // bytes between rows
+  int rows, N, bias_dtype, res_dtype, c_dtype, act;
+  int lg, slack;           // entries of a range: 1 << lg; how far a row may reach behind it
+  bool vec;                // rows of C, residual and preact start on 16-byte boundaries, N is a multiple of 8
 };
 
-// A warp per row, 128 features at a time.
-template <int DT>
-__global__ void __launch_bounds__(256)
-spmm_csr_act_rows_kernel(ActArgs a) {
-  using T = Type<DT>;
-  const int lane = threadIdx.x & 31, f0 = blockIdx.y * 128 + lane;
-  const int64_t base = a.indptr[a.row_begin];
-  for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < a.rows; row += (int64_t)gridDim.x * 8) {
-    const int64_t s0 = a.indptr[a.row_begin + row], s1 = min(a.indptr[a.row_begin + row + 1], base + a.nnz);
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int64_t e = s0; e < s1; ++e) {
-      const int32_t col = a.indices[e];
-      float v = a.data ? a.data[a.order ? a.order[e] : e] : 1.f;
-      if (v == 0.f) continue;
-      if (a.b_scale) v *= a.b_scale[col];
-      const auto* b = reinterpret_cast<const typename T::T*>(a.B) + (int64_t)col * a.ldb;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (f0 + 32 * i < a.N) acc[i] = fmaf(v, T::get(b[f0 + 32 * i]), acc[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int f = f0 + 32 * i;
-      if (f >= a.N) continue;
-      const float z = a.bias ? acc[i] + get_any(a.bias, f, a.bias_dtype) : acc[i];
-      if (a.preact) put_any(a.preact, row * a.ld_pre + f, a.c_dtype, z);
-      float y = activate(z, a.act);
-      if (a.residual) y += get_any(a.residual, row * a.ld_res + f, a.res_dtype);
-      put_any(a.C, row * a.ldc + f, a.c_dtype, y);
+// ---- epilogue ---------------------------------------------------------------------------------------
+__device__ __forceinline__ char* row_at(const void* base, int row, uint32_t pitch) {
+  return reinterpret_cast<char*>(const_cast<void*>(row_of_b(base, (uint32_t)row, pitch)));
+}
+
+// Eight neighbouring features of a residual as they are stored: 16-bit types fill the first half.
+struct Raw8 { uint4 a, b; };
+__device__ __forceinline__ void fetch8(const ActArgs& a, int row, int f, Raw8& r) {
+  if (!a.residual) return;
+  const char* p = row_at(a.residual, row, a.pitch_res);
+  if (a.vec) {
+    if (a.res_dtype == LF_DTYPE_F32) {
+      r.a = __ldcs(reinterpret_cast<const uint4*>(p + f * 4));
+      r.b = __ldcs(reinterpret_cast<const uint4*>(p + f * 4) + 1);
+    } else {
+      r.a = __ldcs(reinterpret_cast<const uint4*>(p + f * 2));
     }
   }
+}
+
+// v[i] = act(v[i]).  The two kinds with a sigmoid share their code: z * sigmoid(z (k0 + k1 z^2)).  The error function takes
+// the eight in turn, since eight copies of it would not stay in the instruction cache.
+__device__ __forceinline__ void activate8(float* v, int act) {
+  if (act == LF_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = max_nan(v[i], 0.f);
+  } else if (act == LF_ACT_SILU || act == LF_ACT_GELU_TANH) {
+    const float k0 = act == LF_ACT_SILU ? 1.f : kGelu0, k1 = act == LF_ACT_SILU ? 0.f : kGelu0 * kGelu1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= sigmoid(v[i] * fmaf(k1 * v[i], v[i], k0));
+  } else if (act == LF_ACT_GELU) {
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      const float z = activate(v[0], LF_ACT_GELU);
+#pragma unroll
+      for (int k = 0; k < 7; ++k) v[k] = v[k + 1];
+      v[7] = z;
+    }
+  }
+}
+
+// z = A * B for eight neighbouring features of a row from f on, `left` of them in the row -> what the call returns.  bias:
+// theirs, r: their residual (fetch8).
+__device__ __forceinline__ void store8(char* p, int f, int dt, const float* v) {
+  if (dt == LF_DTYPE_F32) {
+    float4* q = reinterpret_cast<float4*>(p + f * 4);
+    __stcs(q, make_float4(v[0], v[1], v[2], v[3]));
+    __stcs(q + 1, make_float4(v[4], v[5], v[6], v[7]));
+  } else {
+    uint32_t w[4];
+    if (dt == LF_DTYPE_BF16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<__nv_bfloat162*>(w + i) = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<__half2*>(w + i) = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    }
+    __stcs(reinterpret_cast<uint4*>(p + f * 2), make_uint4(w[0], w[1], w[2], w[3]));
+  }
+}
+__device__ __forceinline__ void finish8(const ActArgs& a, int row, int f, int left, const float* bias, const Raw8& r, float* z) {
+  char* pc = row_at(a.C, row, a.pitch_c);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) z[i] += bias[i];
+  if (a.vec) {
+    if (a.preact) store8(row_at(a.preact, row, a.pitch_pre), f, a.c_dtype, z);
+    activate8(z, a.act);
+    if (a.residual) {
+      const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+      if (a.res_dtype == LF_DTYPE_F32) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) z[k] += __uint_as_float(w[k]);
+      } else if (a.res_dtype == LF_DTYPE_BF16) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          z[2 * k] += __uint_as_float(w[k] << 16);
+          z[2 * k + 1] += __uint_as_float(w[k] & 0xffff0000u);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 x = __half22float2(*reinterpret_cast<const __half2*>(w + k));
+          z[2 * k] += x.x;
+          z[2 * k + 1] += x.y;
+        }
+      }
+    }
+    store8(pc, f, a.c_dtype, z);
+  } else {   // one by one
+    const char* pr = row_at(a.residual, row, a.pitch_res);
+    char* pp = row_at(a.preact, row, a.pitch_pre);
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      if (i < left) {
+        if (a.preact) put_any(pp, f + i, a.c_dtype, z[0]);
+        float y = activate(z[0], a.act);
+        if (a.residual) y += get_any(pr, f + i, a.res_dtype);
+        put_any(pc, f + i, a.c_dtype, y);
+      }
+#pragma unroll
+      for (int k = 0; k < 7; ++k) z[k] = z[k + 1];
+    }
+  }
+}
+
+// ---- the walk ---------------------------------------------------------------------------------------
+// The rows done side by side leave their sums in shared memory, and the warp's lanes take eight features each from there:
+// the outputs' types and alignment ask for one place in the code and whole 16-byte accesses.
+template <int DT, int G, int CH>
+struct ActWork {
+  using S = Share<DT, G, CH>;
+  static_assert(S::kFloats <= 16, "at most two turns");
+  static constexpr int R = 32 / G, kSpan = S::kSpan, kTurns = (R * kSpan + 255) / 256;
+  const ActArgs& a;
+  const float* bias;    // in shared memory, from the walk's first feature on
+  float* out;           // [R][kSpan]
+  int64_t slots;        // of the range in `partial`
+  int f0, nf, g, gl;
+  uint64_t sum[S::kPairs];
+  Raw8 res[kTurns];
+
+  // what the lane does in turn t: a row of those side by side, features from `f` on
+  __device__ __forceinline__ int item(int t) const { return (t * 32 + g * G + gl) / (kSpan / 8); }
+  __device__ __forceinline__ int feature(int t) const { return (t * 32 + g * G + gl) % (kSpan / 8) * 8; }
+
+  __device__ __forceinline__ void coming(int row) const {   // the residual, 128 bytes at a time
+    if (!a.residual) return;
+    const int bytes = dtype_bytes(a.res_dtype);
+    const char* p = row_at(a.residual, row, a.pitch_res) + f0 * bytes;
+    for (int i = 0; i < nf * bytes; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + i));
+  }
+  __device__ __forceinline__ void begin(int row) {
+#pragma unroll
+    for (int i = 0; i < S::kPairs; ++i) sum[i] = 0;
+    if (a.residual) {   // on its way while the row is summed up
+#pragma unroll
+      for (int t = 0; t < kTurns; ++t) {
+        const int r = __shfl_sync(kAllLanes, row, item(t) * G & 31);
+        if (item(t) < R && r >= 0 && feature(t) < nf) fetch8(a, r, f0 + feature(t), res[t]);
+      }
+    }
+  }
+  __device__ __forceinline__ void step(float v, const unsigned char* x) {
+    uint64_t f[S::kPairs];
+    S::floats(x, gl, f);
+    const uint64_t vv = as_pair(__float_as_uint(v), __float_as_uint(v));
+#pragma unroll
+    for (int i = 0; i < S::kPairs; ++i) sum[i] = fma_pair(vv, f[i], sum[i]);
+  }
+  __device__ __forceinline__ void steps_done(int, bool) const {}
+  __device__ __forceinline__ void end(int row, bool whole, int piece) {
+    if (whole) {
+#pragma unroll
+      for (int o = G; o < 32; o <<= 1) {
+#pragma unroll
+        for (int i = 0; i < S::kPairs; ++i) sum[i] = add_pair(sum[i], __shfl_xor_sync(kAllLanes, (unsigned long long)sum[i], o));
+      }
+      if (g > 0) row = -1;
+    }
+    __syncwarp();
+    if constexpr (!S::kShifted) {
+#pragma unroll
+      for (int i = 0; i < S::kFloats; i += 4)
+        *reinterpret_cast<ulonglong2*>(out + g * kSpan + S::feature(i, gl)) = make_ulonglong2(sum[i / 2], sum[i / 2 + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < S::kPairs; ++i) {
+        const float2 p = as_floats(sum[i]);
+        out[g * kSpan + S::feature(2 * i, gl)] = p.x;
+        out[g * kSpan + S::feature(2 * i + 1, gl)] = p.y;
+      }
+    }
+    __syncwarp();
+#pragma unroll 1
+    for (int t = 0; t < kTurns; ++t) {
+      const int r = __shfl_sync(kAllLanes, row, item(t) * G & 31), f = feature(t);
+      if (item(t) < R && r >= 0 && f < nf) {
+      float z[8];
+      const float4* q = reinterpret_cast<const float4*>(out + item(t) * kSpan + f);
+      const float4 x = q[0], y = q[1];
+      z[0] = x.x; z[1] = x.y; z[2] = x.z; z[3] = x.w; z[4] = y.x; z[5] = y.y; z[6] = y.z; z[7] = y.w;
+      if (whole && piece >= 0) {   // a piece: as it is
+        float4* p = reinterpret_cast<float4*>(a.partial + (slots + piece) * a.ld_partial + f0 + f);
+        p[0] = x;
+        p[1] = y;
+      } else {
+        finish8(a, r, f0 + f, nf - f, bias + f, res[0], z);
+      }
+      }
+      res[0] = res[kTurns - 1];   // (an index that is not a constant would put them into memory)
+    }
+  }
+};
+
+template <int DT, int G, int CH, bool IND>
+__global__ void __launch_bounds__(kWalkThreads, 5)
+spmm_csr_act_kernel(const __grid_constant__ ActArgs a) {
+  using S = Share<DT, G, CH>;
+  extern __shared__ __align__(16) unsigned char act_smem[];
+  WalkSmem* walks = reinterpret_cast<WalkSmem*>(act_smem);
+  float* out = reinterpret_cast<float*>(walks + kWalkThreads / 32);
+  float* bias = out + kWalkThreads * S::kFloats;
+  let_dependents_launch();
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int f0 = blockIdx.y * S::kFeatures, nf = min(a.N - f0, S::kFeatures);
+  for (int f = threadIdx.x; f < S::kSpan; f += kWalkThreads) bias[f] = a.bias && f < nf ? get_any(a.bias, f0 + f, a.bias_dtype) : 0.f;
+  __syncthreads();
+  RowStarts ptr;
+  ptr.init(a.indptr, a.rows, a.nnz);
+  const int64_t q = (int64_t)blockIdx.x * (kWalkThreads / 32) + w;
+  if ((q << a.lg) >= ptr.total) return;
+  const WalkArgs wa{a.indices + ptr.base, a.data && !a.order ? a.data + ptr.base : a.data, a.order ? a.order + ptr.base : nullptr, a.b_scale,
+                    reinterpret_cast<const char*>(a.B) + (int64_t)f0 * dtype_bytes(DT), a.pitch_b, nf};
+  ActWork<DT, G, CH> work{a, bias, out + w * (32 * S::kFloats), 2 * q, f0, nf, lane / G, lane % G};
+  RowWalk<DT, G, CH, IND, ActWork<DT, G, CH>>(wa, ptr, walks[w], work).range(q, a.lg, a.slack);
+}
+
+// Rows without entries, and rows that several ranges share: their pieces in order.  A lane has eight features; rows of few pieces
+// are a warp's, rows of many the block's, whose warps take every eighth piece.
+constexpr int kLongPieces = 8;
+
+__device__ __forceinline__ void bias8(const ActArgs& a, int f, float* b) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) b[i] = a.bias && f + i < a.N ? get_any(a.bias, f + i, a.bias_dtype) : 0.f;
+}
+__device__ __forceinline__ void add_piece(const ActArgs& a, int64_t slot, int f, float* z) {
+  const float4* p = reinterpret_cast<const float4*>(a.partial + slot * a.ld_partial + f);
+  const float4 x = __ldcg(p), y = __ldcg(p + 1);
+  z[0] += x.x; z[1] += x.y; z[2] += x.z; z[3] += x.w;
+  z[4] += y.x; z[5] += y.y; z[6] += y.z; z[7] += y.w;
+}
+
+__global__ void __launch_bounds__(kThreads)
+finish_rows_kernel(const __grid_constant__ ActArgs a) {
+  __shared__ int rows_of[kThreads / 32][32], long_rows[kThreads], num_long;
+  __shared__ int64_t starts_of[kThreads / 32][32], ends_of[kThreads / 32][32];
+  __shared__ float sums[kThreads / 32][256 + 8];
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  RowStarts ptr;
+  ptr.init(a.indptr, a.rows, a.nnz);
+  const int chunks = (a.N + 7) / 8;
+  for (int64_t row0 = (int64_t)blockIdx.x * kThreads; row0 < a.rows; row0 += (int64_t)gridDim.x * kThreads) {
+    if (threadIdx.x == 0) num_long = 0;
+    __syncthreads();
+    const int64_t row = row0 + threadIdx.x;
+    int64_t s = 0, e = 0;
+    bool mine = false;
+    if (row < a.rows) {
+      s = ptr((int)row);
+      e = ptr((int)row + 1);
+      mine = s >= e;
+      if (!mine && row_is_cut(s, e, a.lg, a.slack)) {
+        mine = ((e - 1) >> a.lg) - (s >> a.lg) < kLongPieces;
+        if (!mine) long_rows[atomicAdd(&num_long, 1)] = (int)row;   // in any order: each row is one block's from here on
+      }
+    }
+    const unsigned todo = __ballot_sync(kAllLanes, mine);
+    if (mine) {
+      const int i = __popc(todo & ((1u << lane) - 1u));
+      rows_of[w][i] = (int)row;
+      starts_of[w][i] = s;
+      ends_of[w][i] = e;
+    }
+    __syncwarp();
+    wait_for_prior_grid();   // the pieces are there
+    const int per = chunks < 32 ? chunks : 32;   // lanes per row
+    for (int i = lane / per; i < __popc(todo) && lane < 32 / per * per; i += 32 / per) {
+      const int64_t s1 = starts_of[w][i], e1 = ends_of[w][i];
+      for (int c = lane % per; c < chunks; c += per) {
+        float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (s1 < e1) {
+          const int64_t q0 = s1 >> a.lg, q1 = (e1 - 1) >> a.lg;
+          add_piece(a, 2 * q0 + 1, c * 8, z);
+#pragma unroll 8
+          for (int64_t q = q0 + 1; q <= q1; ++q) add_piece(a, 2 * q, c * 8, z);
+        }
+        float bias[8];
+        bias8(a, c * 8, bias);
+        Raw8 r;
+        fetch8(a, rows_of[w][i], c * 8, r);
+        finish8(a, rows_of[w][i], c * 8, a.N - c * 8, bias, r, z);
+      }
+    }
+    __syncthreads();
+    for (int i = 0; i < num_long; ++i) {
+      const int r = long_rows[i];
+      const int64_t q0 = ptr(r) >> a.lg, q1 = (ptr(r + 1) - 1) >> a.lg;
+      for (int f0 = 0; f0 < a.N; f0 += 256) {
+        const int f = f0 + lane * 8;
+        float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (f < a.N) {
+          if (w == 0) add_piece(a, 2 * q0 + 1, f, z);
+#pragma unroll 8
+          for (int64_t q = q0 + 1 + w; q <= q1; q += kThreads / 32) add_piece(a, 2 * q, f, z);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sums[w][lane * 8 + k] = z[k];
+        __syncthreads();
+        if (w == 0 && f < a.N) {
+          for (int v = 1; v < kThreads / 32; ++v) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) z[k] += sums[v][lane * 8 + k];
+          }
+          float bias[8];
+          bias8(a, f, bias);
+          Raw8 old;
+          fetch8(a, r, f, old);
+          finish8(a, r, f, a.N - f, bias, old, z);
+        }
+        __syncthreads();
+      }
+    }
+    __syncthreads();
+  }
+}
+
+template <int DT, int G, int CH, bool IND>
+cudaError_t launch_walk_as(const ActArgs& a, cudaStream_t st) {
+  using S = Share<DT, G, CH>;
+  constexpr auto kernel = spmm_csr_act_kernel<DT, G, CH, IND>;
+  constexpr int smem = kWalkThreads / 32 * (int)sizeof(WalkSmem) + kWalkThreads * S::kFloats * 4 + S::kSpan * 4;
+  const cudaError_t e = allow_smem<kernel>(smem);
+  if (e != cudaSuccess) return e;
+  const dim3 grid((unsigned)ceil_div64(ceil_div64(a.nnz, (int64_t)1 << a.lg), kWalkThreads / 32), (unsigned)((a.N + S::kFeatures - 1) / S::kFeatures));
+  kernel<<<grid, kWalkThreads, smem, st>>>(a);
+  return cudaGetLastError();
+}
+
+template <int DT>
+cudaError_t launch_walk(const ActArgs& a, cudaStream_t st) {
+  return with_row_shape<DT>((uintptr_t)a.B % 16 == 0 && a.pitch_b % 16 == 0, a.N, [&](auto G, auto CH) {
+    if constexpr (DT != LF_DTYPE_E4M3)
+      if (!a.b_scale && !a.order) return launch_walk_as<DT, G.value, CH.value, false>(a, st);
+    return launch_walk_as<DT, G.value, CH.value, true>(a, st);
+  });
 }
 
 }  // namespace
@@ -61,7 +375,10 @@ using namespace lf;
 
 extern "C" {
 
-size_t lf_spmm_csr_act_workspace_bytes(int64_t nnz, int32_t N, int32_t b_dtype) { return 0; }
+size_t lf_spmm_csr_act_workspace_bytes(int64_t nnz, int32_t N, int32_t b_dtype) {
+  if (nnz < 1 || N < 1) return 0;
+  return (size_t)ceil_div64(nnz, (int64_t)1 << range_log(nnz)) * 2 * align_up((size_t)N, 8) * sizeof(float);
+}
 
 int lf_spmm_csr_act(const int64_t* indptr, const int32_t* indices, const float* data, const int32_t* order,
                     int64_t row_begin, int64_t row_end, int64_t nnz, const void* B, int32_t b_dtype, int64_t ldb,
@@ -77,22 +394,33 @@ int lf_spmm_csr_act(const int64_t* indptr, const int32_t* indices, const float* 
   const lf_epilogue& ep = epilogue ? *epilogue : none;
   LF_REQUIRE(ep.activation >= LF_ACT_NONE && ep.activation <= LF_ACT_GELU_TANH, "unknown activation");
   LF_REQUIRE(!ep.bias || is_wide_dtype(ep.bias_dtype), "the bias must be float32, bfloat16 or float16");
-  LF_REQUIRE(!ep.residual || (is_wide_dtype(ep.residual_dtype) && ep.ld_residual >= N), "bad residual");
-  LF_REQUIRE(!ep.preact || ep.ld_preact >= N, "bad leading dimension of preact");
+  LF_REQUIRE(!ep.residual || (is_wide_dtype(ep.residual_dtype) && ep.ld_residual >= N && ep.ld_residual < (1ll << 30)), "bad residual");
+  LF_REQUIRE(!ep.preact || (ep.ld_preact >= N && ep.ld_preact < (1ll << 30)), "bad leading dimension of preact");
   if (row_begin == row_end) return LF_OK;
   LF_REQUIRE(indptr && C, "null pointer argument");
   LF_REQUIRE(nnz == 0 || (indices && B), "indices or B missing");
   LF_REQUIRE(!order || (data && nnz < (1ll << 31)), "order goes with data, for fewer than 2^31 entries");
-  const ActArgs a{indptr, indices, data, order, row_begin, row_end - row_begin, nnz, B, b_scale, ldb, ep.bias, ep.residual,
-                  ep.preact, C, ep.ld_residual, ep.ld_preact, ldc, N, ep.bias_dtype, ep.residual_dtype, c_dtype, ep.activation};
+  const size_t need = lf_spmm_csr_act_workspace_bytes(nnz, N, b_dtype);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(LF_ERR_WORKSPACE_TOO_SMALL, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  LF_REQUIRE((uintptr_t)workspace % 16 == 0, "the workspace must start on a 16-byte boundary");
+  const int lg = range_log(nnz);
+  LF_REQUIRE((nnz >> lg) < (1ll << 31) - 1, "too many entries");
+  const bool vec = N % 8 == 0 && on_grid16(C, ldc, c_dtype) && (!ep.residual || on_grid16(ep.residual, ep.ld_residual, ep.residual_dtype)) &&
+                   (!ep.preact || on_grid16(ep.preact, ep.ld_preact, c_dtype));
+  const ActArgs a{indptr + row_begin, indices, data, order, nnz, B, b_scale, ep.bias, ep.residual, ep.preact, C, (float*)workspace,
+                  (int64_t)align_up((size_t)N, 8), (uint32_t)ldb * dtype_bytes(b_dtype), (uint32_t)ep.ld_residual * dtype_bytes(ep.residual_dtype),
+                  (uint32_t)ep.ld_preact * dtype_bytes(c_dtype), (uint32_t)ldc * dtype_bytes(c_dtype), (int)(row_end - row_begin), N,
+                  ep.bias_dtype, ep.residual_dtype, c_dtype, ep.activation, lg, range_slack(lg), vec};
   cudaStream_t st = (cudaStream_t)stream;
-  const int64_t blocks = ceil_div64(a.rows, 8);
-  const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20), (unsigned)((N + 127) / 128));
-  if (b_dtype == LF_DTYPE_F32) spmm_csr_act_rows_kernel<LF_DTYPE_F32><<<grid, 256, 0, st>>>(a);
-  else if (b_dtype == LF_DTYPE_BF16) spmm_csr_act_rows_kernel<LF_DTYPE_BF16><<<grid, 256, 0, st>>>(a);
-  else if (b_dtype == LF_DTYPE_F16) spmm_csr_act_rows_kernel<LF_DTYPE_F16><<<grid, 256, 0, st>>>(a);
-  else spmm_csr_act_rows_kernel<LF_DTYPE_E4M3><<<grid, 256, 0, st>>>(a);
-  LF_CUDA_CHECK(cudaGetLastError());
+  if (nnz > 0) {
+    if (b_dtype == LF_DTYPE_F32) LF_CUDA_CHECK(launch_walk<LF_DTYPE_F32>(a, st));
+    else if (b_dtype == LF_DTYPE_BF16) LF_CUDA_CHECK(launch_walk<LF_DTYPE_BF16>(a, st));
+    else if (b_dtype == LF_DTYPE_F16) LF_CUDA_CHECK(launch_walk<LF_DTYPE_F16>(a, st));
+    else LF_CUDA_CHECK(launch_walk<LF_DTYPE_E4M3>(a, st));
+  }
+  const int64_t blocks = ceil_div64(a.rows, kThreads);
+  LF_CUDA_CHECK(launch_dep(finish_rows_kernel, dim3((unsigned)(blocks < (1 << 16) ? blocks : 1 << 16)), kThreads, st, nnz > 0, a));
   return LF_OK;
 }
 

@@ -224,7 +224,7 @@ class CsrTranspose:
 
 
 def _product(lib, a, data, order, r0, r1, nnz, B, b_code, ldb, scale_ptr, out, ldc, N, ep, workspace, dev):
-    nbytes = lib.lf_spmm_csr_act_workspace_bytes(a.nnz, N, b_code)
+    nbytes = lib.lf_spmm_csr_act_workspace_bytes(nnz, N, b_code)
     keep, ws = _scratch(nbytes, workspace, B.device)
     check(lib.lf_spmm_csr_act(a.indptr.data_ptr(), a.indices.data_ptr(), data, order, r0, r1, nnz, B.data_ptr(), b_code, ldb,
                               scale_ptr, out.data_ptr(), _code(out.dtype), ldc, N, ep, ws, nbytes, stream_of(dev)))

@@ -68,6 +68,15 @@ def test_product_refusals(kw):
     assert product(**kw) == BAD
 
 
+@pytest.mark.parametrize("kw", [dict(ws=0), dict(nws=63)])
+def test_product_workspace(kw):
+    assert product(**kw) == SMALL
+
+
+def test_product_workspace_off_the_grid():
+    assert product(ws=P + 4) == BAD
+
+
 def test_product_of_no_rows_does_nothing():
     assert product(r1=0, indptr=0, C=0) == 0
 
@@ -112,7 +121,7 @@ def test_workspace_queries_are_pure():
     assert lib.lf_rms_norm_backward_workspace_bytes(1000, 8) >= 32
     assert lib.lf_act_backward_workspace_bytes(1000, 8) >= 32
     sizes = [lib.lf_spmm_csr_act_workspace_bytes(n, 64, BF16) for n in (0, 1, 1000, 10 ** 6, 10 ** 8)]
-    assert sizes == sorted(sizes)
+    assert sizes == sorted(sizes) and sizes[0] == 0
 
 
 @pytest.mark.parametrize("shape,seed", [((0, 5), 0), ((5, 0), 0), ((1, 1), 1), ((7, 12), 2), ((60, 31), 3)])
