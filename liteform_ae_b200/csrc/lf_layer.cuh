@@ -160,6 +160,33 @@ __device__ __forceinline__ float activate_slope(float z, int act) {
   }
 }
 
+// v[i] = act'(v[i]) for n values; the error function's slope four at a time in turn, to keep the code short
+template <int n>
+__device__ __forceinline__ void slopes(float* v, int act) {
+  if (act == LF_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < n; ++i) v[i] = activate_slope(v[i], LF_ACT_RELU);
+  } else if (act == LF_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < n; ++i) v[i] = activate_slope(v[i], LF_ACT_SILU);
+  } else if (act == LF_ACT_GELU_TANH) {
+#pragma unroll
+    for (int i = 0; i < n; ++i) v[i] = activate_slope(v[i], LF_ACT_GELU_TANH);
+  } else if (act == LF_ACT_GELU) {
+    constexpr int k = n < 4 ? n : 4;
+#pragma unroll 1
+    for (int t = 0; t < n; t += k) {
+      float z[k];
+#pragma unroll
+      for (int i = 0; i < k; ++i) z[i] = activate_slope(v[i], LF_ACT_GELU);
+#pragma unroll
+      for (int i = 0; i < n - k; ++i) v[i] = v[i + k];
+#pragma unroll
+      for (int i = 0; i < k; ++i) v[n - k + i] = z[i];
+    }
+  }
+}
+
 __device__ __forceinline__ float warp_sum(float v) {   // the same sum in every lane
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

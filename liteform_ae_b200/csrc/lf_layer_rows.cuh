@@ -191,7 +191,7 @@ struct WalkArgs {
   int nf;                  // features from there on, at most kFeatures
 };
 
-constexpr int kWalkThreads = 128;
+constexpr int kWalkThreads = 64;    // two warps: a block ends with the slower of two ranges (four: 3 % more on the graph above)
 constexpr int kWindow = 256;        // entries of the rows taken at a time, rows rounded up to fours
 constexpr int kShortRow = 32;       // longest row that one group does
 constexpr int kAtOnce = 4;          // steps (a row of B per group) that are copied and added up together
@@ -202,7 +202,7 @@ struct WalkSmem {
   unsigned char ring[kRingBytes + 16];   // shifted rows are read up to their shift past the ring's end
   __align__(16) uint32_t col[kWindow];   // or with the mark; a group's row, or its share of one, from a multiple of four on
   float val[kWindow];
-  int32_t sorted[32];                    // rows of the window that have entries, the shortest first
+  int32_t sorted[32];                    // rows of the window that have entries, the shortest first: number, place, size in fours
 };
 
 // Copies the lane's pieces of a row of B into the ring (PIECES of 16 bytes, `STRIDE` apart in the row), those that are
@@ -227,7 +227,9 @@ __device__ __forceinline__ void copy_row(uint32_t dst, const void* src, uint32_t
 
 // A walk over the rows of one range.  IND: there may be scales or an order.  `Work` has
 //   coming(row)              a row of the window, by one of its lanes
-//   begin(row)               every group begins a row (row < 0: the group has none to write), or all groups the same one
+//   begin(row, whole, piece, at, end)   every group begins a row (row < 0: the group has none), or, `whole`, all groups the
+//                            same one; its entries are at places below `end`, and the one at place p is entry at + p (both
+//                            only where Work::kPlaces)
 //   step(val, x)             an entry of the row (one that the group does not have has the value 0): x is the lane's share of
 //                            its row of B, as Share::floats takes it
 //   steps_done(k, in)        after four steps: k is the place of the first of them in the window; in: they are the group's
@@ -251,7 +253,8 @@ struct RowWalk {
 
   // A group's row (or -1) and its places in the window, in fours; steps: the longest row's of the groups.
   struct Batch {
-    int row, from, own, steps;
+    int row, from, own, steps, end;
+    int64_t at;
     __device__ __forceinline__ bool has(int k) const { return k < own; }
     __device__ __forceinline__ int place(int k) const { return has(k) ? from + k * U : 0; }
   };
@@ -408,7 +411,7 @@ struct RowWalk {
         }
         __syncwarp();
         if (size > 0) {
-          sm.sorted[place] = lane;
+          sm.sorted[place] = lane | from << 8 | size << 20;
           work.coming(row + lane);
         }
         after = ptr(row + rows + lane + 1);
@@ -422,6 +425,7 @@ struct RowWalk {
         __syncwarp();
       }
       stage(e, places, [&](int i) {   // place i is of the last row that starts at or before it
+        if (left > 0) return i < n ? i : -1;
         int of = 0;
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1)
@@ -436,14 +440,17 @@ struct RowWalk {
       auto batch = [&](int p) {
         Batch b;
         if (whole) {
-          b = {row, g * share, share / U, share / U};
+          b = {row, g * share, share / U, share / U, n, e};
         } else {
-          const int mine = p + g < held ? sm.sorted[p + g] : -1, of = sm.sorted[min(p + R, held) - 1];   // of: the longest
-          b.steps = __shfl_sync(kAllLanes, size, of);
-          b.from = __shfl_sync(kAllLanes, from, mine < 0 ? of : mine);
-          b.own = __shfl_sync(kAllLanes, size, mine < 0 ? of : mine);
-          b.row = mine < 0 ? -1 : row + mine;
-          if (mine < 0) b.own = 0;
+          const int mine = p + g < held ? sm.sorted[p + g] : 0;
+          b.own = mine >> 20;
+          b.row = b.own > 0 ? row + (mine & 31) : -1;
+          b.from = (mine >> 8) & 0xfff;
+          b.steps = sm.sorted[min(p + R, held) - 1] >> 20;
+          if constexpr (Work::kPlaces) {
+            b.end = b.from + __shfl_sync(kAllLanes, length, mine & 31);
+            b.at = e + __shfl_sync(kAllLanes, first, mine & 31) - b.from;
+          }
         }
         return b;
       };
@@ -466,7 +473,7 @@ struct RowWalk {
 #pragma unroll 1
       for (int p = 0; p < held; p += R) {
         const Batch now = batch(p);
-        if (!whole || !begun) work.begin(whole && (g > 0 || piece >= 0) ? -1 : now.row);
+        if (!whole || !begun || Work::kPlaces) work.begin(now.row, whole, piece, now.at, now.end);
 #pragma unroll 1
         for (int k = 0; k < now.steps; ++k) {
           take(now.place(k), now.has(k));

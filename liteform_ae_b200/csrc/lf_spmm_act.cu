@@ -36,149 +36,183 @@ __device__ __forceinline__ char* row_at(const void* base, int row, uint32_t pitc
   return reinterpret_cast<char*>(const_cast<void*>(row_of_b(base, (uint32_t)row, pitch)));
 }
 
-// Eight neighbouring features of a residual as they are stored: 16-bit types fill the first half.
-struct Raw8 { uint4 a, b; };
-__device__ __forceinline__ void fetch8(const ActArgs& a, int row, int f, Raw8& r) {
-  if (!a.residual) return;
-  const char* p = row_at(a.residual, row, a.pitch_res);
-  if (a.vec) {
-    if (a.res_dtype == LF_DTYPE_F32) {
-      r.a = __ldcs(reinterpret_cast<const uint4*>(p + f * 4));
-      r.b = __ldcs(reinterpret_cast<const uint4*>(p + f * 4) + 1);
-    } else {
-      r.a = __ldcs(reinterpret_cast<const uint4*>(p + f * 2));
-    }
-  }
-}
-
 // v[i] = act(v[i]).  The two kinds with a sigmoid share their code: z * sigmoid(z (k0 + k1 z^2)).  The error function takes
-// the eight in turn, since eight copies of it would not stay in the instruction cache.
-__device__ __forceinline__ void activate8(float* v, int act) {
+// four at a time in turn, since a copy of it for each would not stay in the instruction cache.
+template <int n>
+__device__ __forceinline__ void activate_all(float* v, int act) {
   if (act == LF_ACT_RELU) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = max_nan(v[i], 0.f);
+    for (int i = 0; i < n; ++i) v[i] = max_nan(v[i], 0.f);
   } else if (act == LF_ACT_SILU || act == LF_ACT_GELU_TANH) {
     const float k0 = act == LF_ACT_SILU ? 1.f : kGelu0, k1 = act == LF_ACT_SILU ? 0.f : kGelu0 * kGelu1;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= sigmoid(v[i] * fmaf(k1 * v[i], v[i], k0));
+    for (int i = 0; i < n; ++i) v[i] *= sigmoid(v[i] * fmaf(k1 * v[i], v[i], k0));
   } else if (act == LF_ACT_GELU) {
 #pragma unroll 1
-    for (int i = 0; i < 8; ++i) {
-      const float z = activate(v[0], LF_ACT_GELU);
+    for (int i = 0; i < n; i += 4) {
+      float z[4];
 #pragma unroll
-      for (int k = 0; k < 7; ++k) v[k] = v[k + 1];
-      v[7] = z;
+      for (int k = 0; k < 4; ++k) z[k] = activate(v[k], LF_ACT_GELU);
+#pragma unroll
+      for (int k = 0; k < n - 4; ++k) v[k] = v[k + 4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[n - 4 + k] = z[k];
     }
   }
 }
 
-// z = A * B for eight neighbouring features of a row from f on, `left` of them in the row -> what the call returns.  bias:
-// theirs, r: their residual (fetch8).
-__device__ __forceinline__ void store8(char* p, int f, int dt, const float* v) {
-  if (dt == LF_DTYPE_F32) {
-    float4* q = reinterpret_cast<float4*>(p + f * 4);
-    __stcs(q, make_float4(v[0], v[1], v[2], v[3]));
-    __stcs(q + 1, make_float4(v[4], v[5], v[6], v[7]));
-  } else {
-    uint32_t w[4];
-    if (dt == LF_DTYPE_BF16) {
+// What a lane has of a row: BLOCKS of n neighbouring features, `apart` from one block to the next, `left` of them from the
+// first on to the row's end.  vec: the row is on the 16-byte grid and holds whole eights, so blocks move as they are, and
+// `w` holds them as they are stored; otherwise one by one, and `w` holds floats.
+template <int BLOCKS, int n>
+struct RowIo {
+  static __device__ __forceinline__ void load(const char* p, int dt, bool vec, int apart, int left, uint32_t* w) {
+    if (vec) {
+      const int bytes = dtype_bytes(dt);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) *reinterpret_cast<__nv_bfloat162*>(w + i) = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      for (int b = 0; b < BLOCKS; ++b) {
+        if (b * apart >= left) break;
+        const char* q = p + b * apart * bytes;
+        if (dt == LF_DTYPE_F32) {
+#pragma unroll
+          for (int i = 0; i < n; i += 4) *reinterpret_cast<uint4*>(w + b * n + i) = __ldcs(reinterpret_cast<const uint4*>(q + i * 4));
+        } else if (n == 4) {
+          *reinterpret_cast<uint2*>(w + b * n) = __ldcs(reinterpret_cast<const uint2*>(q));
+        } else {
+#pragma unroll
+          for (int i = 0; i < n; i += 8) *reinterpret_cast<uint4*>(w + b * n + i / 2) = __ldcs(reinterpret_cast<const uint4*>(q + i * 2));
+        }
+      }
+    } else if constexpr (BLOCKS * n <= 4) {
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) {
+#pragma unroll
+        for (int i = 0; i < n; ++i)
+          if (b * apart + i < left) w[b * n + i] = __float_as_uint(get_any(p, b * apart + i, dt));
+      }
+    } else {   // (in memory, not to have the code once for each)
+      uint32_t t[BLOCKS * n];
+#pragma unroll 1
+      for (int i = 0; i < BLOCKS * n; ++i)
+        if (i / n * apart + i % n < left) t[i] = __float_as_uint(get_any(p, i / n * apart + i % n, dt));
+#pragma unroll
+      for (int i = 0; i < BLOCKS * n; ++i) w[i] = t[i];
+    }
+  }
+  static __device__ __forceinline__ void add(const uint32_t* w, int dt, bool vec, float* v) {
+    if (!vec || dt == LF_DTYPE_F32) {
+#pragma unroll
+      for (int i = 0; i < BLOCKS * n; ++i) v[i] += __uint_as_float(w[i]);
+    } else if (dt == LF_DTYPE_BF16) {
+#pragma unroll
+      for (int i = 0; i < BLOCKS * n; ++i) {
+        const uint32_t h = w[i / n * n + i % n / 2];
+        v[i] += __uint_as_float(i & 1 ? h & 0xffff0000u : h << 16);
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) *reinterpret_cast<__half2*>(w + i) = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-    }
-    __stcs(reinterpret_cast<uint4*>(p + f * 2), make_uint4(w[0], w[1], w[2], w[3]));
-  }
-}
-__device__ __forceinline__ void finish8(const ActArgs& a, int row, int f, int left, const float* bias, const Raw8& r, float* z) {
-  char* pc = row_at(a.C, row, a.pitch_c);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) z[i] += bias[i];
-  if (a.vec) {
-    if (a.preact) store8(row_at(a.preact, row, a.pitch_pre), f, a.c_dtype, z);
-    activate8(z, a.act);
-    if (a.residual) {
-      const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
-      if (a.res_dtype == LF_DTYPE_F32) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) z[k] += __uint_as_float(w[k]);
-      } else if (a.res_dtype == LF_DTYPE_BF16) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          z[2 * k] += __uint_as_float(w[k] << 16);
-          z[2 * k + 1] += __uint_as_float(w[k] & 0xffff0000u);
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 x = __half22float2(*reinterpret_cast<const __half2*>(w + k));
-          z[2 * k] += x.x;
-          z[2 * k + 1] += x.y;
-        }
+      for (int i = 0; i < BLOCKS * n; i += 2) {
+        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(w + i / n * n + i % n / 2));
+        v[i] += x.x;
+        v[i + 1] += x.y;
       }
     }
-    store8(pc, f, a.c_dtype, z);
-  } else {   // one by one
-    const char* pr = row_at(a.residual, row, a.pitch_res);
-    char* pp = row_at(a.preact, row, a.pitch_pre);
+  }
+  static __device__ __forceinline__ void store(char* p, int dt, bool vec, int apart, int left, const float* v) {
+    if (vec) {
+      const int bytes = dtype_bytes(dt);
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) {
+        if (b * apart >= left) break;
+        char* q = p + b * apart * bytes;
+        if (dt == LF_DTYPE_F32) {
+#pragma unroll
+          for (int i = 0; i < n; i += 4) __stcs(reinterpret_cast<float4*>(q + i * 4), make_float4(v[b * n + i], v[b * n + i + 1], v[b * n + i + 2], v[b * n + i + 3]));
+        } else {
+          uint32_t h[n / 2 > 0 ? n / 2 : 1];
+#pragma unroll
+          for (int i = 0; i < n; i += 2) {
+            if (dt == LF_DTYPE_BF16) *reinterpret_cast<__nv_bfloat162*>(h + i / 2) = __floats2bfloat162_rn(v[b * n + i], v[b * n + i + 1]);
+            else *reinterpret_cast<__half2*>(h + i / 2) = __floats2half2_rn(v[b * n + i], v[b * n + i + 1]);
+          }
+          if constexpr (n == 4) {
+            __stcs(reinterpret_cast<uint2*>(q), make_uint2(h[0], h[1]));
+          } else {
+#pragma unroll
+            for (int i = 0; i < n / 2; i += 4) __stcs(reinterpret_cast<uint4*>(q + i * 4), make_uint4(h[i], h[i + 1], h[i + 2], h[i + 3]));
+          }
+        }
+      }
+    } else if constexpr (BLOCKS * n <= 4) {
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) {
+#pragma unroll
+        for (int i = 0; i < n; ++i)
+          if (b * apart + i < left) put_any(p, b * apart + i, dt, v[b * n + i]);
+      }
+    } else {
+      float t[BLOCKS * n];
+#pragma unroll
+      for (int i = 0; i < BLOCKS * n; ++i) t[i] = v[i];
 #pragma unroll 1
-    for (int i = 0; i < 8; ++i) {
-      if (i < left) {
-        if (a.preact) put_any(pp, f + i, a.c_dtype, z[0]);
-        float y = activate(z[0], a.act);
-        if (a.residual) y += get_any(pr, f + i, a.res_dtype);
-        put_any(pc, f + i, a.c_dtype, y);
-      }
-#pragma unroll
-      for (int k = 0; k < 7; ++k) z[k] = z[k + 1];
+      for (int i = 0; i < BLOCKS * n; ++i)
+        if (i / n * apart + i % n < left) put_any(p, i / n * apart + i % n, dt, t[i]);
     }
   }
+  // z = A * B for features f on, `bias` theirs, w their residual -> what the call returns
+  static __device__ __forceinline__ void finish(const ActArgs& a, bool vec, int row, int f, int apart, int left, const float* bias, const uint32_t* w, float* z) {
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+#pragma unroll
+      for (int i = 0; i < n; ++i) z[b * n + i] += bias[b * apart + i];
+    }
+    const int at = f * dtype_bytes(a.c_dtype);
+    if (a.preact) store(row_at(a.preact, row, a.pitch_pre) + at, a.c_dtype, vec, apart, left, z);
+    activate_all<BLOCKS * n>(z, a.act);
+    if (a.residual) add(w, a.res_dtype, vec, z);
+    store(row_at(a.C, row, a.pitch_c) + at, a.c_dtype, vec, apart, left, z);
+  }
+};
+// eight features, the residual fetched here
+__device__ __forceinline__ void finish8(const ActArgs& a, int row, int f, const float* bias, float* z) {
+  __align__(16) uint32_t w[8];
+  if (a.residual) RowIo<1, 8>::load(row_at(a.residual, row, a.pitch_res) + f * dtype_bytes(a.res_dtype), a.res_dtype, a.vec, 8, a.N - f, w);
+  RowIo<1, 8>::finish(a, a.vec, row, f, 8, a.N - f, bias, w, z);
 }
 
 // ---- the walk ---------------------------------------------------------------------------------------
-// The rows done side by side leave their sums in shared memory, and the warp's lanes take eight features each from there:
-// the outputs' types and alignment ask for one place in the code and whole 16-byte accesses.
 template <int DT, int G, int CH>
 struct ActWork {
   using S = Share<DT, G, CH>;
-  static_assert(S::kFloats <= 16, "at most two turns");
-  static constexpr int R = 32 / G, kSpan = S::kSpan, kTurns = (R * kSpan + 255) / 256;
+  // the lane's share of a row in memory
+  static constexpr int kBlocks = S::kShifted ? S::kFloats : S::kPieces, kBlock = S::kFloats / kBlocks, kApart = S::kShifted ? G : G * S::VEC;
+  using Io = RowIo<kBlocks, kBlock>;
   const ActArgs& a;
-  const float* bias;    // in shared memory, from the walk's first feature on
-  float* out;           // [R][kSpan]
+  const float* bias;    // in shared memory, from the lane's first feature on
   int64_t slots;        // of the range in `partial`
-  int f0, nf, g, gl;
+  int f, left, gl;      // the lane's first feature; features from there to the end of the walk
+  bool vec;
   uint64_t sum[S::kPairs];
-  Raw8 res[kTurns];
-
-  // what the lane does in turn t: a row of those side by side, features from `f` on
-  __device__ __forceinline__ int item(int t) const { return (t * 32 + g * G + gl) / (kSpan / 8); }
-  __device__ __forceinline__ int feature(int t) const { return (t * 32 + g * G + gl) % (kSpan / 8) * 8; }
+  __align__(16) uint32_t res[S::kFloats];
 
   __device__ __forceinline__ void coming(int row) const {   // the residual, 128 bytes at a time
     if (!a.residual) return;
-    const int bytes = dtype_bytes(a.res_dtype);
-    const char* p = row_at(a.residual, row, a.pitch_res) + f0 * bytes;
-    for (int i = 0; i < nf * bytes; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + i));
+    const char* p = row_at(a.residual, row, a.pitch_res);
+    for (int i = 0; i < (int)(a.N * dtype_bytes(a.res_dtype)); i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + i));
   }
-  __device__ __forceinline__ void begin(int row) {
+  static constexpr bool kPlaces = false;
+  __device__ __forceinline__ void begin(int row, bool whole, int piece, int64_t, int) {
 #pragma unroll
     for (int i = 0; i < S::kPairs; ++i) sum[i] = 0;
-    if (a.residual) {   // on its way while the row is summed up
-#pragma unroll
-      for (int t = 0; t < kTurns; ++t) {
-        const int r = __shfl_sync(kAllLanes, row, item(t) * G & 31);
-        if (item(t) < R && r >= 0 && feature(t) < nf) fetch8(a, r, f0 + feature(t), res[t]);
-      }
-    }
+    if (a.residual && row >= 0 && !(whole && piece >= 0))   // on its way while the row is summed up
+      Io::load(row_at(a.residual, row, a.pitch_res) + f * dtype_bytes(a.res_dtype), a.res_dtype, vec, kApart, left, res);
   }
   __device__ __forceinline__ void step(float v, const unsigned char* x) {
-    uint64_t f[S::kPairs];
-    S::floats(x, gl, f);
+    uint64_t y[S::kPairs];
+    S::floats(x, gl, y);
     const uint64_t vv = as_pair(__float_as_uint(v), __float_as_uint(v));
 #pragma unroll
-    for (int i = 0; i < S::kPairs; ++i) sum[i] = fma_pair(vv, f[i], sum[i]);
+    for (int i = 0; i < S::kPairs; ++i) sum[i] = fma_pair(vv, y[i], sum[i]);
   }
   __device__ __forceinline__ void steps_done(int, bool) const {}
   __device__ __forceinline__ void end(int row, bool whole, int piece) {
@@ -188,51 +222,34 @@ struct ActWork {
 #pragma unroll
         for (int i = 0; i < S::kPairs; ++i) sum[i] = add_pair(sum[i], __shfl_xor_sync(kAllLanes, (unsigned long long)sum[i], o));
       }
-      if (g > 0) row = -1;
+      if ((threadIdx.x & 31) >= G) return;
     }
-    __syncwarp();
-    if constexpr (!S::kShifted) {
+    if (row < 0) return;
+    float z[S::kFloats];
 #pragma unroll
-      for (int i = 0; i < S::kFloats; i += 4)
-        *reinterpret_cast<ulonglong2*>(out + g * kSpan + S::feature(i, gl)) = make_ulonglong2(sum[i / 2], sum[i / 2 + 1]);
+    for (int i = 0; i < S::kPairs; ++i) {
+      const float2 p = as_floats(sum[i]);
+      z[2 * i] = p.x;
+      z[2 * i + 1] = p.y;
+    }
+    if (whole && piece >= 0) {   // as it is
+      float* p = a.partial + (slots + piece) * a.ld_partial + f;
+#pragma unroll
+      for (int i = 0; i < S::kFloats; ++i)
+        if (i / kBlock * kApart + i % kBlock < left) p[i / kBlock * kApart + i % kBlock] = z[i];
     } else {
-#pragma unroll
-      for (int i = 0; i < S::kPairs; ++i) {
-        const float2 p = as_floats(sum[i]);
-        out[g * kSpan + S::feature(2 * i, gl)] = p.x;
-        out[g * kSpan + S::feature(2 * i + 1, gl)] = p.y;
-      }
-    }
-    __syncwarp();
-#pragma unroll 1
-    for (int t = 0; t < kTurns; ++t) {
-      const int r = __shfl_sync(kAllLanes, row, item(t) * G & 31), f = feature(t);
-      if (item(t) < R && r >= 0 && f < nf) {
-      float z[8];
-      const float4* q = reinterpret_cast<const float4*>(out + item(t) * kSpan + f);
-      const float4 x = q[0], y = q[1];
-      z[0] = x.x; z[1] = x.y; z[2] = x.z; z[3] = x.w; z[4] = y.x; z[5] = y.y; z[6] = y.z; z[7] = y.w;
-      if (whole && piece >= 0) {   // a piece: as it is
-        float4* p = reinterpret_cast<float4*>(a.partial + (slots + piece) * a.ld_partial + f0 + f);
-        p[0] = x;
-        p[1] = y;
-      } else {
-        finish8(a, r, f0 + f, nf - f, bias + f, res[0], z);
-      }
-      }
-      res[0] = res[kTurns - 1];   // (an index that is not a constant would put them into memory)
+      Io::finish(a, vec, row, f, kApart, left, bias, res, z);
     }
   }
 };
 
 template <int DT, int G, int CH, bool IND>
-__global__ void __launch_bounds__(kWalkThreads, 5)
+__global__ void __launch_bounds__(kWalkThreads, 640 / kWalkThreads)
 spmm_csr_act_kernel(const __grid_constant__ ActArgs a) {
   using S = Share<DT, G, CH>;
   extern __shared__ __align__(16) unsigned char act_smem[];
   WalkSmem* walks = reinterpret_cast<WalkSmem*>(act_smem);
-  float* out = reinterpret_cast<float*>(walks + kWalkThreads / 32);
-  float* bias = out + kWalkThreads * S::kFloats;
+  float* bias = reinterpret_cast<float*>(walks + kWalkThreads / 32);
   let_dependents_launch();
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int f0 = blockIdx.y * S::kFeatures, nf = min(a.N - f0, S::kFeatures);
@@ -244,7 +261,8 @@ spmm_csr_act_kernel(const __grid_constant__ ActArgs a) {
   if ((q << a.lg) >= ptr.total) return;
   const WalkArgs wa{a.indices + ptr.base, a.data && !a.order ? a.data + ptr.base : a.data, a.order ? a.order + ptr.base : nullptr, a.b_scale,
                     reinterpret_cast<const char*>(a.B) + (int64_t)f0 * dtype_bytes(DT), a.pitch_b, nf};
-  ActWork<DT, G, CH> work{a, bias, out + w * (32 * S::kFloats), 2 * q, f0, nf, lane / G, lane % G};
+  const int first = S::feature(0, lane % G);
+  ActWork<DT, G, CH> work{a, bias + first, 2 * q, f0 + first, nf - first, lane % G, !S::kShifted && a.vec && a.N % ActWork<DT, G, CH>::kBlock == 0};
   RowWalk<DT, G, CH, IND, ActWork<DT, G, CH>>(wa, ptr, walks[w], work).range(q, a.lg, a.slack);
 }
 
@@ -309,9 +327,7 @@ finish_rows_kernel(const __grid_constant__ ActArgs a) {
         }
         float bias[8];
         bias8(a, c * 8, bias);
-        Raw8 r;
-        fetch8(a, rows_of[w][i], c * 8, r);
-        finish8(a, rows_of[w][i], c * 8, a.N - c * 8, bias, r, z);
+        finish8(a, rows_of[w][i], c * 8, bias, z);
       }
     }
     __syncthreads();
@@ -336,9 +352,7 @@ finish_rows_kernel(const __grid_constant__ ActArgs a) {
           }
           float bias[8];
           bias8(a, f, bias);
-          Raw8 old;
-          fetch8(a, r, f, old);
-          finish8(a, r, f, a.N - f, bias, old, z);
+          finish8(a, r, f, bias, z);
         }
         __syncthreads();
       }
@@ -351,7 +365,7 @@ template <int DT, int G, int CH, bool IND>
 cudaError_t launch_walk_as(const ActArgs& a, cudaStream_t st) {
   using S = Share<DT, G, CH>;
   constexpr auto kernel = spmm_csr_act_kernel<DT, G, CH, IND>;
-  constexpr int smem = kWalkThreads / 32 * (int)sizeof(WalkSmem) + kWalkThreads * S::kFloats * 4 + S::kSpan * 4;
+  constexpr int smem = kWalkThreads / 32 * (int)sizeof(WalkSmem) + S::kSpan * 4;
   const cudaError_t e = allow_smem<kernel>(smem);
   if (e != cudaSuccess) return e;
   const dim3 grid((unsigned)ceil_div64(ceil_div64(a.nnz, (int64_t)1 << a.lg), kWalkThreads / 32), (unsigned)((a.N + S::kFeatures - 1) / S::kFeatures));

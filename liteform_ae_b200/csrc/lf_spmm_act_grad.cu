@@ -1,6 +1,8 @@
 // Gradients of Y = act(A * B + bias) + residual besides that of B (which is the product with A transposed):
 // dZ = dY * act'(Z), its sum over the rows for the bias, and the gradient of A's values.
-#include "lf_layer.cuh"
+#include <type_traits>
+
+#include "lf_layer_rows.cuh"
 
 namespace lf {
 
@@ -8,70 +10,212 @@ cudaError_t launch_column_sum(const float* partial, int parts, int N, float* out
 
 namespace {
 
+// ---- dZ and the bias --------------------------------------------------------------------------------
 struct ActGradArgs {
   const void* dy;
   const void* z;       // or NULL: no activation
   void* dz;            // or NULL
   float* partial;      // [parts][N], or NULL
   int64_t rows, ld_dy, ld_z, ld_dz;
-  int N, act, rows_per_part;
+  int N, act;
+  int per_row;         // threads per row, a power of two
 };
 
-template <int DT>
+// A block's threads are 256 / per_row rows side by side, VEC features each; a thread keeps its features while it walks down
+// the rows, so that the bias's sum stays in registers.  The inputs are read once and dZ is written once: memory bounds it,
+// and, with the error function's slope, the instructions (2^18 rows of 256 bfloat16: see the table of measurements).
+template <int DT, int VEC>
 __global__ void __launch_bounds__(256)
 act_grad_kernel(ActGradArgs a) {
-  using T = Type<DT>;
-  const int f = blockIdx.y * 256 + threadIdx.x;
-  if (f >= a.N) return;
-  const int64_t r0 = (int64_t)blockIdx.x * a.rows_per_part, r1 = min(r0 + a.rows_per_part, a.rows);
-  float s = 0.f;
-  for (int64_t r = r0; r < r1; ++r) {
-    float d = T::get(reinterpret_cast<const typename T::T*>(a.dy)[r * a.ld_dy + f]);
-    if (a.z) d *= activate_slope(T::get(reinterpret_cast<const typename T::T*>(a.z)[r * a.ld_z + f]), a.act);
-    if (a.dz) reinterpret_cast<typename T::T*>(a.dz)[r * a.ld_dz + f] = T::put(d);
-    s += d;
-  }
-  if (a.partial) a.partial[(int64_t)blockIdx.x * a.N + f] = s;
-}
-
-struct ValueGradArgs {
-  const int64_t* indptr;
-  const int32_t* indices;
-  int64_t row_begin, rows, nnz;
-  const void* dy;
-  const void* z;
-  const void* B;
-  float* dvalues;
-  int64_t ld_dy, ld_z, ldb;
-  int N, act, dy_dtype;
-};
-
-// A warp per row.
-template <int DT>
-__global__ void __launch_bounds__(256)
-value_grad_rows_kernel(ValueGradArgs a) {
-  using T = Type<DT>;
-  const int lane = threadIdx.x & 31;
-  const int64_t base = a.indptr[a.row_begin];
-  for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < a.rows; row += (int64_t)gridDim.x * 8) {
-    const int64_t s0 = a.indptr[a.row_begin + row], s1 = min(a.indptr[a.row_begin + row + 1], base + a.nnz);
-    for (int64_t e = s0; e < s1; ++e) {
-      const auto* b = reinterpret_cast<const typename T::T*>(a.B) + (int64_t)a.indices[e] * a.ldb;
-      float s = 0.f;
-      for (int f = lane; f < a.N; f += 32) {
-        float d = get_any(a.dy, row * a.ld_dy + f, a.dy_dtype);
-        if (a.z) d *= activate_slope(get_any(a.z, row * a.ld_z + f, a.dy_dtype), a.act);
-        s = fmaf(d, T::get(b[f]), s);
+  using E = typename Type<DT>::T;
+  __shared__ float sums[256 * VEC];
+  const int t = threadIdx.x % a.per_row, r = threadIdx.x / a.per_row, side = 256 / a.per_row;
+  const int f = (blockIdx.y * a.per_row + t) * VEC;
+  float s[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) s[i] = 0.f;
+  if (f < a.N) {
+#pragma unroll 2
+    for (int64_t row = (int64_t)blockIdx.x * side + r; row < a.rows; row += (int64_t)gridDim.x * side) {
+      Pack<DT, VEC> d, z;
+      d.fetch(reinterpret_cast<const E*>(a.dy) + row * a.ld_dy + f);
+      if (a.z) z.fetch(reinterpret_cast<const E*>(a.z) + row * a.ld_z + f);
+      float v[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = a.z ? z.get(i) : 0.f;
+      if (a.z) slopes<VEC>(v, a.act);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        v[i] = a.z ? d.get(i) * v[i] : d.get(i);
+        s[i] += v[i];
       }
-      s = warp_sum(s);
-      if (lane == 0) a.dvalues[e - base] = s;
+      if (a.dz) {
+        Pack<DT, VEC> o;
+        o.put(v);
+        o.keep(reinterpret_cast<E*>(a.dz) + row * a.ld_dz + f);   // gathered next
+      }
     }
   }
+  if (!a.partial) return;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) sums[threadIdx.x * VEC + i] = s[i];
+  __syncthreads();
+  const int width = a.per_row * VEC;
+  for (int i = threadIdx.x; i < width; i += 256) {
+    float v = sums[i];
+    for (int k = 1; k < side; ++k) v += sums[k * width + i];
+    if (blockIdx.y * width + i < a.N) a.partial[(int64_t)blockIdx.x * a.N + blockIdx.y * width + i] = v;
+  }
 }
 
-constexpr int kParts = 1184;   // 148 SMs x 8
+constexpr int kMostParts = 148 * 6;
 
-int rows_per_part(int64_t rows) { return (int)ceil_div64(rows, kParts); }
+// ---- gradient of the values -------------------------------------------------------------------------
+struct ValueGradArgs {
+  const int64_t* indptr;   // of row_begin
+  const int32_t* indices;
+  int64_t nnz;
+  const void* dy;
+  const void* z;           // or NULL: no activation
+  const void* B;
+  float* dvalues;          // first of the row range's entries
+  uint32_t pitch_dy, pitch_z, pitch_b;
+  int rows, N, dy_dtype, act, lg, slack, f0;
+};
+
+// The group keeps its row of dZ in registers (computed there, not rounded) and multiplies the rows of B that come through the
+// ring with it; four dot products at a time are summed up over the lanes, each lane ending with one of them.  A row wider
+// than a walk takes several launches, which add to what the ones before wrote.
+template <int DT, int G, int CH>
+struct GradWork {
+  using S = Share<DT, G, CH>;
+  static constexpr bool kPlaces = true;
+  static constexpr int kVec = S::kShifted ? 1 : S::VEC, kApart = S::kShifted ? G : G * S::VEC;
+  const ValueGradArgs& a;
+  int f, left, gl;
+  bool ragged;             // the row's last piece of 16 bytes is not full
+  int stop, used;
+  int64_t at;
+  uint64_t dz[S::kPairs];
+  float dot[kAtOnce];
+
+  __device__ __forceinline__ void coming(int row) const {
+    prefetch(a.dy, row, a.pitch_dy);
+    if (a.z) prefetch(a.z, row, a.pitch_z);
+  }
+  __device__ __forceinline__ void prefetch(const void* base, int row, uint32_t pitch) const {
+    const char* p = reinterpret_cast<const char*>(row_of_b(base, (uint32_t)row, pitch));
+    for (int i = 0; i < a.N * dtype_bytes(a.dy_dtype); i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + i));
+  }
+  // the lane's features of a row, as floats; 0 behind its end
+  __device__ __forceinline__ void load(const void* base, int row, uint32_t pitch, float* v) const {
+    const char* p = reinterpret_cast<const char*>(row_of_b(base, (uint32_t)row, pitch)) + f * dtype_bytes(a.dy_dtype);
+    if (a.dy_dtype == LF_DTYPE_F32) {
+#pragma unroll
+      for (int i = 0; i < S::kFloats; ++i) {
+        const int k = i / kVec * kApart + i % kVec;
+        v[i] = k < left ? __ldg(reinterpret_cast<const float*>(p) + k) : 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < S::kFloats; ++i) {
+        const int k = i / kVec * kApart + i % kVec;
+        const uint32_t h = k < left ? __ldg(reinterpret_cast<const uint16_t*>(p) + k) : 0u;
+        v[i] = a.dy_dtype == LF_DTYPE_BF16 ? __uint_as_float(h << 16) : __half2float(__ushort_as_half((unsigned short)h));
+      }
+    }
+  }
+  __device__ __forceinline__ void begin(int row, bool, int, int64_t at_, int end_) {
+    at = at_;
+    stop = end_;
+    used = 0;
+    float d[S::kFloats];
+    if (row >= 0) {
+      load(a.dy, row, a.pitch_dy, d);
+      if (a.z) {
+        float z[S::kFloats];
+        load(a.z, row, a.pitch_z, z);
+        slopes<S::kFloats>(z, a.act);
+#pragma unroll
+        for (int i = 0; i < S::kFloats; ++i)
+          d[i] = i / kVec * kApart + i % kVec < left ? d[i] * z[i] : 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < S::kFloats; ++i) d[i] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < S::kPairs; ++i) dz[i] = as_pair(__float_as_uint(d[2 * i]), __float_as_uint(d[2 * i + 1]));
+  }
+  __device__ __forceinline__ void step(float, const unsigned char* x) {
+    uint64_t y[S::kPairs], s = 0;
+    S::floats(x, gl, y);
+    // What lies behind the row's end may be anything, and a 0 in dz does not make up for it.
+    constexpr int kPart = S::kShifted ? 1 : S::VEC / 2;   // pairs that are there or not together, but for a ragged end
+#pragma unroll
+    for (int c = 0; c < S::kPairs; c += kPart) {
+      if (2 * c / kVec * kApart >= left) continue;
+#pragma unroll
+      for (int i = c; i < c + kPart; ++i) {
+        if (ragged) {
+          const int k = 2 * i / kVec * kApart + 2 * i % kVec, k1 = (2 * i + 1) / kVec * kApart + (2 * i + 1) % kVec;
+          const float2 p = as_floats(y[i]);
+          y[i] = as_pair(k < left ? __float_as_uint(p.x) : 0u, k1 < left ? __float_as_uint(p.y) : 0u);
+        }
+        s = fma_pair(dz[i], y[i], s);
+      }
+    }
+    dot[used++ % kAtOnce] = as_floats(s).x + as_floats(s).y;
+  }
+  __device__ __forceinline__ void steps_done(int place, bool in) {
+    used = 0;
+    // lane gl ends with the dot product of place + (gl & 3)
+    const bool up = gl & 2, odd = gl & 1;
+    float k0 = up ? dot[2] : dot[0], k1 = up ? dot[3] : dot[1];
+    k0 += __shfl_xor_sync(kAllLanes, up ? dot[0] : dot[2], 2);
+    k1 += __shfl_xor_sync(kAllLanes, up ? dot[1] : dot[3], 2);
+    float s = odd ? k1 : k0;
+    s += __shfl_xor_sync(kAllLanes, odd ? k0 : k1, 1);
+#pragma unroll
+    for (int o = 4; o < G; o <<= 1) s += __shfl_xor_sync(kAllLanes, s, o);
+    if (in && gl < 4 && place + gl < stop) {
+      float* p = a.dvalues + at + place + gl;
+      *p = a.f0 > 0 ? *p + s : s;
+    }
+  }
+  __device__ __forceinline__ void end(int, bool, int) const {}
+};
+
+template <int DT, int G, int CH>
+__global__ void __launch_bounds__(kWalkThreads, 640 / kWalkThreads)
+value_grad_kernel(const __grid_constant__ ValueGradArgs a) {
+  using S = Share<DT, G, CH>;
+  extern __shared__ __align__(16) unsigned char grad_smem[];
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, first = S::feature(0, lane % G);
+  const int nf = min(a.N - a.f0, S::kFeatures);
+  RowStarts ptr;
+  ptr.init(a.indptr, a.rows, a.nnz);
+  const int64_t q = (int64_t)blockIdx.x * (kWalkThreads / 32) + w;
+  if ((q << a.lg) >= ptr.total) return;
+  const WalkArgs wa{a.indices + ptr.base, nullptr, nullptr, nullptr, reinterpret_cast<const char*>(a.B) + (int64_t)a.f0 * dtype_bytes(DT), a.pitch_b, nf};
+  GradWork<DT, G, CH> work{a, a.f0 + first, nf - first, lane % G, S::kShifted || a.N % S::VEC != 0};
+  RowWalk<DT, G, CH, false, GradWork<DT, G, CH>>(wa, ptr, reinterpret_cast<WalkSmem*>(grad_smem)[w], work).range(q, a.lg, a.slack);
+}
+
+template <int DT>
+cudaError_t launch_value_grad(ValueGradArgs a, cudaStream_t st) {
+  return with_row_shape<DT>((uintptr_t)a.B % 16 == 0 && a.pitch_b % 16 == 0, a.N, [&](auto G, auto CH) {
+    constexpr auto kernel = value_grad_kernel<DT, G.value, CH.value>;
+    constexpr int smem = kWalkThreads / 32 * (int)sizeof(WalkSmem);
+    cudaError_t e = allow_smem<kernel>(smem);
+    const unsigned grid = (unsigned)ceil_div64(ceil_div64(a.nnz, (int64_t)1 << a.lg), kWalkThreads / 32);
+    for (a.f0 = 0; a.f0 < a.N && e == cudaSuccess; a.f0 += Share<DT, G.value, CH.value>::kFeatures) {
+      kernel<<<grid, kWalkThreads, smem, st>>>(a);
+      e = cudaGetLastError();
+    }
+    return e;
+  });
+}
 
 }  // namespace
 }  // namespace lf
@@ -82,7 +226,7 @@ extern "C" {
 
 size_t lf_act_backward_workspace_bytes(int64_t rows, int32_t N) {
   if (rows < 1 || N < 1) return 0;
-  return (size_t)ceil_div64(rows, rows_per_part(rows)) * (size_t)N * sizeof(float);
+  return (size_t)(rows < kMostParts ? rows : kMostParts) * (size_t)N * sizeof(float);
 }
 
 int lf_act_backward(const void* dy, int64_t ld_dy, const void* preact, int64_t ld_preact, int32_t dtype,
@@ -102,13 +246,22 @@ int lf_act_backward(const void* dy, int64_t ld_dy, const void* preact, int64_t l
   if (dbias && (!workspace || workspace_bytes < lf_act_backward_workspace_bytes(rows, N)))
     return fail(LF_ERR_WORKSPACE_TOO_SMALL, "workspace of %zu bytes, %zu needed", workspace_bytes,
                 lf_act_backward_workspace_bytes(rows, N));
-  const ActGradArgs a{dy, activation == LF_ACT_NONE ? nullptr : preact, dz, dbias ? (float*)workspace : nullptr,
-                      rows, ld_dy, ld_preact, ld_dz, N, activation, rows_per_part(rows)};
-  const int parts = (int)ceil_div64(rows, a.rows_per_part);
-  const dim3 grid((unsigned)parts, (unsigned)((N + 255) / 256));
-  if (dtype == LF_DTYPE_F32) act_grad_kernel<LF_DTYPE_F32><<<grid, 256, 0, st>>>(a);
-  else if (dtype == LF_DTYPE_BF16) act_grad_kernel<LF_DTYPE_BF16><<<grid, 256, 0, st>>>(a);
-  else act_grad_kernel<LF_DTYPE_F16><<<grid, 256, 0, st>>>(a);
+  const void* z = activation == LF_ACT_NONE ? nullptr : preact;
+  const int per = 16 / dtype_bytes(dtype);
+  const bool vec = N % per == 0 && on_grid16(dy, ld_dy, dtype) && (!z || on_grid16(z, ld_preact, dtype)) && (!dz || on_grid16(dz, ld_dz, dtype));
+  const int pieces = vec ? N / per : N;
+  int per_row = 4;
+  while (per_row < pieces && per_row < 256) per_row *= 2;
+  const ActGradArgs a{dy, z, dz, dbias ? (float*)workspace : nullptr, rows, ld_dy, ld_preact, ld_dz, N, activation, per_row};
+  const int64_t want = ceil_div64(rows, 256 / per_row);
+  const int parts = (int)(want < kMostParts ? want : kMostParts);
+  const dim3 grid((unsigned)parts, (unsigned)((pieces + per_row - 1) / per_row));
+  LF_REQUIRE(grid.y < 65536, "too many features");
+#define LF_GO(DT_, VEC_) act_grad_kernel<DT_, VEC_><<<grid, 256, 0, st>>>(a)
+  if (dtype == LF_DTYPE_F32) { if (vec) LF_GO(LF_DTYPE_F32, 4); else LF_GO(LF_DTYPE_F32, 1); }
+  else if (dtype == LF_DTYPE_BF16) { if (vec) LF_GO(LF_DTYPE_BF16, 8); else LF_GO(LF_DTYPE_BF16, 1); }
+  else { if (vec) LF_GO(LF_DTYPE_F16, 8); else LF_GO(LF_DTYPE_F16, 1); }
+#undef LF_GO
   LF_CUDA_CHECK(cudaGetLastError());
   if (dbias) LF_CUDA_CHECK(launch_column_sum(a.partial, parts, N, dbias, st));
   return LF_OK;
@@ -125,15 +278,16 @@ int lf_spmm_csr_grad_values(const int64_t* indptr, const int32_t* indices, int64
   if (row_begin == row_end || nnz == 0) return LF_OK;
   LF_REQUIRE(indptr && indices && dy && B && dvalues, "null pointer argument");
   LF_REQUIRE(activation == LF_ACT_NONE || (preact && ld_preact >= N && ld_preact < (1ll << 30)), "preact missing");
-  const ValueGradArgs a{indptr, indices, row_begin, row_end - row_begin, nnz, dy, activation == LF_ACT_NONE ? nullptr : preact,
-                        B, dvalues, ld_dy, ld_preact, ldb, N, activation, dy_dtype};
+  const int lg = range_log(nnz);
+  LF_REQUIRE((nnz >> lg) < (1ll << 31) - 1, "too many entries");
+  const uint32_t bytes = (uint32_t)dtype_bytes(dy_dtype);
+  const ValueGradArgs a{indptr + row_begin, indices, nnz, dy, activation == LF_ACT_NONE ? nullptr : preact, B, dvalues,
+                        (uint32_t)ld_dy * bytes, (uint32_t)ld_preact * bytes, (uint32_t)ldb * dtype_bytes(b_dtype),
+                        (int)(row_end - row_begin), N, dy_dtype, activation, lg, range_slack(lg), 0};
   cudaStream_t st = (cudaStream_t)stream;
-  const int64_t blocks = ceil_div64(a.rows, 8);
-  const unsigned grid = (unsigned)(blocks < (1 << 20) ? blocks : 1 << 20);
-  if (b_dtype == LF_DTYPE_F32) value_grad_rows_kernel<LF_DTYPE_F32><<<grid, 256, 0, st>>>(a);
-  else if (b_dtype == LF_DTYPE_BF16) value_grad_rows_kernel<LF_DTYPE_BF16><<<grid, 256, 0, st>>>(a);
-  else value_grad_rows_kernel<LF_DTYPE_F16><<<grid, 256, 0, st>>>(a);
-  LF_CUDA_CHECK(cudaGetLastError());
+  if (b_dtype == LF_DTYPE_F32) LF_CUDA_CHECK(launch_value_grad<LF_DTYPE_F32>(a, st));
+  else if (b_dtype == LF_DTYPE_BF16) LF_CUDA_CHECK(launch_value_grad<LF_DTYPE_BF16>(a, st));
+  else LF_CUDA_CHECK(launch_value_grad<LF_DTYPE_F16>(a, st));
   return LF_OK;
 }
 
