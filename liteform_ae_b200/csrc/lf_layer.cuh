@@ -126,63 +126,75 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either 
 }
 
 // ---- activations ------------------------------------------------------------------------------------
-// 1 / (1 + exp(-z)); for z so low that the exponential overflows, 0
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + expf(-z)); }
+// 2^x and 1 / x by the special function unit, results below the normal numbers as 0: one instruction each
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+// 1 / (1 + exp(-z)); for z so low that the exponential overflows, 0.  Rounding -z log2(e) makes the exponential's error grow
+// with |z|, as the rounding of z itself does; where it matters the exponential is small beside the 1.
+__device__ __forceinline__ float sigmoid(float z) { return rcp_approx(1.f + exp2_approx(-kLog2e * z)); }
 // the tanh form of GELU is z * sigmoid(gelu_arg(z)), since (1 + tanh u) / 2 = sigmoid(2 u)
 constexpr float kGelu0 = 1.5957691216057308f, kGelu1 = 0.044715f;
 __device__ __forceinline__ float gelu_arg(float z) { return z * fmaf(kGelu0 * kGelu1 * z, z, kGelu0); }
 
-__device__ __forceinline__ float activate(float z, int act) {
-  switch (act) {
-    case LF_ACT_RELU: return max_nan(z, 0.f);
-    case LF_ACT_SILU: return z * sigmoid(z);
-    case LF_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    case LF_ACT_GELU_TANH: return z * sigmoid(gelu_arg(z));
-    default: return z;
-  }
+// (1 + erf(z / sqrt 2)) / 2 and e = exp(-z^2 / 2), which the density takes too: Abramowitz and Stegun 7.1.26, off by at
+// most 7.5e-8 (erff and expf: 40 instructions for 16, 2^18 rows of 256 gradients 142 us for 82)
+__device__ __forceinline__ float normal_cdf(float z, float* e) {
+  const float t = rcp_approx(fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.f));
+  *e = exp2_approx(-0.5f * kLog2e * z * z);
+  const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+  const float q = 0.5f * p * *e;   // of the tail beyond |z|
+  return z < 0.f ? q : 1.f - q;    // a NaN stays one
 }
 
-// beyond +-100 every slope is 0 or 1 to the last bit; so far the formulas stay clear of 0 * infinity
-__device__ __forceinline__ float activate_slope(float z, int act) {
-  z = z > 100.f ? 100.f : z < -100.f ? -100.f : z;
-  switch (act) {
-    case LF_ACT_RELU: return z > 0.f ? 1.f : 0.f;
-    case LF_ACT_SILU: {
-      const float p = sigmoid(z);
-      return p * fmaf(z, 1.f - p, 1.f);
-    }
-    case LF_ACT_GELU: return fmaf(0.5f, erff(z * 0.70710678118654752f), 0.5f) + z * 0.3989422804014327f * expf(-0.5f * z * z);
-    case LF_ACT_GELU_TANH: {
-      const float p = sigmoid(gelu_arg(z));
-      return p * fmaf(z * (1.f - p), 1.5957691216057308f * fmaf(0.134145f * z, z, 1.f), 1.f);
-    }
-    default: return 1.f;
-  }
-}
-
-// v[i] = act'(v[i]) for n values; the error function's slope four at a time in turn, to keep the code short
+// v[i] = act(v[i]) for n values.  The two kinds with a sigmoid share their code: z * sigmoid(z (k0 + k1 z^2)).
 template <int n>
-__device__ __forceinline__ void slopes(float* v, int act) {
+__device__ __forceinline__ void activate_all(float* v, int act) {
   if (act == LF_ACT_RELU) {
 #pragma unroll
-    for (int i = 0; i < n; ++i) v[i] = activate_slope(v[i], LF_ACT_RELU);
-  } else if (act == LF_ACT_SILU) {
+    for (int i = 0; i < n; ++i) v[i] = max_nan(v[i], 0.f);
+  } else if (act == LF_ACT_SILU || act == LF_ACT_GELU_TANH) {
+    const float k0 = act == LF_ACT_SILU ? 1.f : kGelu0, k1 = act == LF_ACT_SILU ? 0.f : kGelu0 * kGelu1;
 #pragma unroll
-    for (int i = 0; i < n; ++i) v[i] = activate_slope(v[i], LF_ACT_SILU);
-  } else if (act == LF_ACT_GELU_TANH) {
-#pragma unroll
-    for (int i = 0; i < n; ++i) v[i] = activate_slope(v[i], LF_ACT_GELU_TANH);
+    for (int i = 0; i < n; ++i) v[i] *= sigmoid(v[i] * fmaf(k1 * v[i], v[i], k0));
   } else if (act == LF_ACT_GELU) {
-    constexpr int k = n < 4 ? n : 4;
-#pragma unroll 1
-    for (int t = 0; t < n; t += k) {
-      float z[k];
 #pragma unroll
-      for (int i = 0; i < k; ++i) z[i] = activate_slope(v[i], LF_ACT_GELU);
+    for (int i = 0; i < n; ++i) {
+      float e;
+      v[i] *= normal_cdf(v[i], &e);
+    }
+  }
+}
+
+// v[i] = act'(v[i]).  Beyond +-100 every slope is 0 or 1 to the last bit; so far the formulas stay clear of 0 * infinity.
+template <int n>
+__device__ __forceinline__ void slopes(float* v, int act) {
 #pragma unroll
-      for (int i = 0; i < n - k; ++i) v[i] = v[i + k];
+  for (int i = 0; i < n; ++i) v[i] = -max_nan(-max_nan(v[i], -100.f), -100.f);
+  if (act == LF_ACT_RELU) {
 #pragma unroll
-      for (int i = 0; i < k; ++i) v[n - k + i] = z[i];
+    for (int i = 0; i < n; ++i) v[i] = v[i] > 0.f ? 1.f : 0.f;
+  } else if (act == LF_ACT_SILU || act == LF_ACT_GELU_TANH) {
+    const float k0 = act == LF_ACT_SILU ? 1.f : kGelu0, k1 = act == LF_ACT_SILU ? 0.f : kGelu0 * kGelu1;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {   // u = z (k0 + k1 z^2): p + z p (1 - p) u'
+      const float z = v[i], zz = k1 * z * z, p = sigmoid(z * (k0 + zz));
+      v[i] = p * fmaf(z * (1.f - p), fmaf(3.f, zz, k0), 1.f);
+    }
+  } else if (act == LF_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      float e;
+      const float c = normal_cdf(v[i], &e);
+      v[i] = fmaf(0.3989422804014327f * v[i], e, c);
     }
   }
 }

@@ -18,15 +18,16 @@
 
 namespace lf {
 
-// Entries of a warp's range: the most that still gives each of the chip's 148 SMs 48 warps, from 32 to 1024.
+// Entries of a warp's range: the most that still gives each of the chip's 148 SMs the 20 warps that it holds, three times
+// over where there are enough, from 64 to 1024.
 inline int range_log(int64_t nnz) {
   int lg = 10;
-  while (lg > 5 && (nnz >> lg) < 148 * 48) --lg;
+  while (lg > 6 && (nnz >> lg) < 148 * 20 * (lg > 8 ? 3 : 1)) --lg;
   return lg;
 }
 // A row that starts in a range and ends at most so far behind its nominal end belongs to it whole; only longer ones are
 // cut, at the nominal ends.  Their pieces are added up in order by a later launch.
-inline int range_slack(int lg) { return 1 << (lg - 2); }
+inline int range_slack(int lg) { return lg > 7 ? 1 << (lg - 2) : 32; }
 __device__ __forceinline__ bool row_is_cut(int64_t a, int64_t b, int lg, int slack) { return b > (((a >> lg) + 1) << lg) + slack; }
 
 // Row pointers of a row range, relative to its first entry and never beyond the `nnz` the caller gave, so that what
@@ -177,6 +178,48 @@ inline cudaError_t with_row_shape(bool grid16, int N, F&& go) {
     LF_GO(32, 1);
   }
 #undef LF_GO
+}
+
+// BLOCKS of n neighbouring elements of a row in memory, `apart` from one block to the next, as they are stored: `left` of them
+// from the first on to the row's end.  Blocks of 16 bytes and halves of them move as they are.
+template <int BLOCKS, int n>
+__device__ __forceinline__ void load_blocks(const char* p, int dt, int apart, int left, uint32_t* w) {
+  const int bytes = dtype_bytes(dt);
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b) {
+    if (b * apart >= left) break;
+    const char* q = p + b * apart * bytes;
+    if (dt == LF_DTYPE_F32) {
+#pragma unroll
+      for (int i = 0; i < n; i += 4) *reinterpret_cast<uint4*>(w + b * n + i) = __ldcs(reinterpret_cast<const uint4*>(q + i * 4));
+    } else if (n == 4) {
+      *reinterpret_cast<uint2*>(w + b * n) = __ldcs(reinterpret_cast<const uint2*>(q));
+    } else {
+#pragma unroll
+      for (int i = 0; i < n; i += 8) *reinterpret_cast<uint4*>(w + b * n + i / 2) = __ldcs(reinterpret_cast<const uint4*>(q + i * 2));
+    }
+  }
+}
+// v[i] = op(v[i], the element)
+template <int BLOCKS, int n, class Op>
+__device__ __forceinline__ void use_blocks(const uint32_t* w, int dt, float* v, Op op) {
+  if (dt == LF_DTYPE_F32) {
+#pragma unroll
+    for (int i = 0; i < BLOCKS * n; ++i) v[i] = op(v[i], __uint_as_float(w[i]));
+  } else if (dt == LF_DTYPE_BF16) {
+#pragma unroll
+    for (int i = 0; i < BLOCKS * n; ++i) {
+      const uint32_t h = w[i / n * n + i % n / 2];
+      v[i] = op(v[i], __uint_as_float(i & 1 ? h & 0xffff0000u : h << 16));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < BLOCKS * n; i += 2) {
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(w + i / n * n + i % n / 2));
+      v[i] = op(v[i], x.x);
+      if (i + 1 < BLOCKS * n) v[i + 1] = op(v[i + 1], x.y);
+    }
+  }
 }
 
 // ---- the walk ---------------------------------------------------------------------------------------------------
@@ -425,7 +468,7 @@ struct RowWalk {
         __syncwarp();
       }
       stage(e, places, [&](int i) {   // place i is of the last row that starts at or before it
-        if (left > 0) return i < n ? i : -1;
+        if (left > 0 || places == n) return i < n ? i : -1;   // (no row was rounded up)
         int of = 0;
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1)

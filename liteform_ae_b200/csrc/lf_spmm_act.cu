@@ -36,31 +36,6 @@ __device__ __forceinline__ char* row_at(const void* base, int row, uint32_t pitc
   return reinterpret_cast<char*>(const_cast<void*>(row_of_b(base, (uint32_t)row, pitch)));
 }
 
-// v[i] = act(v[i]).  The two kinds with a sigmoid share their code: z * sigmoid(z (k0 + k1 z^2)).  The error function takes
-// four at a time in turn, since a copy of it for each would not stay in the instruction cache.
-template <int n>
-__device__ __forceinline__ void activate_all(float* v, int act) {
-  if (act == LF_ACT_RELU) {
-#pragma unroll
-    for (int i = 0; i < n; ++i) v[i] = max_nan(v[i], 0.f);
-  } else if (act == LF_ACT_SILU || act == LF_ACT_GELU_TANH) {
-    const float k0 = act == LF_ACT_SILU ? 1.f : kGelu0, k1 = act == LF_ACT_SILU ? 0.f : kGelu0 * kGelu1;
-#pragma unroll
-    for (int i = 0; i < n; ++i) v[i] *= sigmoid(v[i] * fmaf(k1 * v[i], v[i], k0));
-  } else if (act == LF_ACT_GELU) {
-#pragma unroll 1
-    for (int i = 0; i < n; i += 4) {
-      float z[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) z[k] = activate(v[k], LF_ACT_GELU);
-#pragma unroll
-      for (int k = 0; k < n - 4; ++k) v[k] = v[k + 4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[n - 4 + k] = z[k];
-    }
-  }
-}
-
 // What a lane has of a row: BLOCKS of n neighbouring features, `apart` from one block to the next, `left` of them from the
 // first on to the row's end.  vec: the row is on the 16-byte grid and holds whole eights, so blocks move as they are, and
 // `w` holds them as they are stored; otherwise one by one, and `w` holds floats.
@@ -68,21 +43,7 @@ template <int BLOCKS, int n>
 struct RowIo {
   static __device__ __forceinline__ void load(const char* p, int dt, bool vec, int apart, int left, uint32_t* w) {
     if (vec) {
-      const int bytes = dtype_bytes(dt);
-#pragma unroll
-      for (int b = 0; b < BLOCKS; ++b) {
-        if (b * apart >= left) break;
-        const char* q = p + b * apart * bytes;
-        if (dt == LF_DTYPE_F32) {
-#pragma unroll
-          for (int i = 0; i < n; i += 4) *reinterpret_cast<uint4*>(w + b * n + i) = __ldcs(reinterpret_cast<const uint4*>(q + i * 4));
-        } else if (n == 4) {
-          *reinterpret_cast<uint2*>(w + b * n) = __ldcs(reinterpret_cast<const uint2*>(q));
-        } else {
-#pragma unroll
-          for (int i = 0; i < n; i += 8) *reinterpret_cast<uint4*>(w + b * n + i / 2) = __ldcs(reinterpret_cast<const uint4*>(q + i * 2));
-        }
-      }
+      load_blocks<BLOCKS, n>(p, dt, apart, left, w);
     } else if constexpr (BLOCKS * n <= 4) {
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b) {
@@ -100,23 +61,7 @@ struct RowIo {
     }
   }
   static __device__ __forceinline__ void add(const uint32_t* w, int dt, bool vec, float* v) {
-    if (!vec || dt == LF_DTYPE_F32) {
-#pragma unroll
-      for (int i = 0; i < BLOCKS * n; ++i) v[i] += __uint_as_float(w[i]);
-    } else if (dt == LF_DTYPE_BF16) {
-#pragma unroll
-      for (int i = 0; i < BLOCKS * n; ++i) {
-        const uint32_t h = w[i / n * n + i % n / 2];
-        v[i] += __uint_as_float(i & 1 ? h & 0xffff0000u : h << 16);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < BLOCKS * n; i += 2) {
-        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(w + i / n * n + i % n / 2));
-        v[i] += x.x;
-        v[i + 1] += x.y;
-      }
-    }
+    use_blocks<BLOCKS, n>(w, vec ? dt : LF_DTYPE_F32, v, [](float x, float y) { return x + y; });
   }
   static __device__ __forceinline__ void store(char* p, int dt, bool vec, int apart, int left, const float* v) {
     if (vec) {
@@ -282,7 +227,7 @@ __device__ __forceinline__ void add_piece(const ActArgs& a, int64_t slot, int f,
 }
 
 __global__ void __launch_bounds__(kThreads)
-finish_rows_kernel(const __grid_constant__ ActArgs a) {
+finish_rows_kernel(const __grid_constant__ ActArgs a, int span) {   // span: rows of a block at a time, at most its threads
   __shared__ int rows_of[kThreads / 32][32], long_rows[kThreads], num_long;
   __shared__ int64_t starts_of[kThreads / 32][32], ends_of[kThreads / 32][32];
   __shared__ float sums[kThreads / 32][256 + 8];
@@ -290,13 +235,13 @@ finish_rows_kernel(const __grid_constant__ ActArgs a) {
   RowStarts ptr;
   ptr.init(a.indptr, a.rows, a.nnz);
   const int chunks = (a.N + 7) / 8;
-  for (int64_t row0 = (int64_t)blockIdx.x * kThreads; row0 < a.rows; row0 += (int64_t)gridDim.x * kThreads) {
+  for (int64_t row0 = (int64_t)blockIdx.x * span; row0 < a.rows; row0 += (int64_t)gridDim.x * span) {
     if (threadIdx.x == 0) num_long = 0;
     __syncthreads();
     const int64_t row = row0 + threadIdx.x;
     int64_t s = 0, e = 0;
     bool mine = false;
-    if (row < a.rows) {
+    if (row < a.rows && threadIdx.x < span) {
       s = ptr((int)row);
       e = ptr((int)row + 1);
       mine = s >= e;
@@ -433,8 +378,12 @@ int lf_spmm_csr_act(const int64_t* indptr, const int32_t* indices, const float* 
     else if (b_dtype == LF_DTYPE_F16) LF_CUDA_CHECK(launch_walk<LF_DTYPE_F16>(a, st));
     else LF_CUDA_CHECK(launch_walk<LF_DTYPE_E4M3>(a, st));
   }
-  const int64_t blocks = ceil_div64(a.rows, kThreads);
-  LF_CUDA_CHECK(launch_dep(finish_rows_kernel, dim3((unsigned)(blocks < (1 << 16) ? blocks : 1 << 16)), kThreads, st, nnz > 0, a));
+  // few rows per block while that fills the chip: a block's long rows are done one after the other (16384 rows, 64 of them
+  // with 2048 entries: 35 us with 256 rows a block, 8 with 32)
+  int span = 32;
+  while (span < kThreads && a.rows > (int64_t)span * 148 * 8) span *= 2;
+  const int64_t blocks = ceil_div64(a.rows, span);
+  LF_CUDA_CHECK(launch_dep(finish_rows_kernel, dim3((unsigned)(blocks < (1 << 16) ? blocks : 1 << 16)), kThreads, st, nnz > 0, a, span));
   return LF_OK;
 }
 

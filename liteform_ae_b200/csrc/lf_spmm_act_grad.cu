@@ -81,6 +81,7 @@ struct ValueGradArgs {
   float* dvalues;          // first of the row range's entries
   uint32_t pitch_dy, pitch_z, pitch_b;
   int rows, N, dy_dtype, act, lg, slack, f0;
+  bool vec;
 };
 
 // The group keeps its row of dZ in registers (computed there, not rounded) and multiplies the rows of B that come through the
@@ -93,7 +94,7 @@ struct GradWork {
   static constexpr int kVec = S::kShifted ? 1 : S::VEC, kApart = S::kShifted ? G : G * S::VEC;
   const ValueGradArgs& a;
   int f, left, gl;
-  bool ragged;             // the row's last piece of 16 bytes is not full
+  bool ragged, vec;        // the row's last piece of 16 bytes is not full; rows of dy and z are on the 16-byte grid
   int stop, used;
   int64_t at;
   uint64_t dz[S::kPairs];
@@ -107,9 +108,17 @@ struct GradWork {
     const char* p = reinterpret_cast<const char*>(row_of_b(base, (uint32_t)row, pitch));
     for (int i = 0; i < a.N * dtype_bytes(a.dy_dtype); i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + i));
   }
-  // the lane's features of a row, as floats; 0 behind its end
+  // the lane's features of a row, as floats; what lies behind its end is anything
   __device__ __forceinline__ void load(const void* base, int row, uint32_t pitch, float* v) const {
     const char* p = reinterpret_cast<const char*>(row_of_b(base, (uint32_t)row, pitch)) + f * dtype_bytes(a.dy_dtype);
+    if (vec) {
+      __align__(16) uint32_t w[S::kFloats];
+      if constexpr (!S::kShifted) {
+        load_blocks<S::kPieces, S::VEC>(p, a.dy_dtype, kApart, left, w);
+        use_blocks<S::kPieces, S::VEC>(w, a.dy_dtype, v, [](float, float y) { return y; });
+      }
+      return;
+    }
     if (a.dy_dtype == LF_DTYPE_F32) {
 #pragma unroll
       for (int i = 0; i < S::kFloats; ++i) {
@@ -137,9 +146,11 @@ struct GradWork {
         load(a.z, row, a.pitch_z, z);
         slopes<S::kFloats>(z, a.act);
 #pragma unroll
-        for (int i = 0; i < S::kFloats; ++i)
-          d[i] = i / kVec * kApart + i % kVec < left ? d[i] * z[i] : 0.f;
+        for (int i = 0; i < S::kFloats; ++i) d[i] *= z[i];
       }
+#pragma unroll
+      for (int i = 0; i < S::kFloats; ++i)
+        if (i / kVec * kApart + i % kVec >= left) d[i] = 0.f;
     } else {
 #pragma unroll
       for (int i = 0; i < S::kFloats; ++i) d[i] = 0.f;
@@ -150,21 +161,23 @@ struct GradWork {
   __device__ __forceinline__ void step(float, const unsigned char* x) {
     uint64_t y[S::kPairs], s = 0;
     S::floats(x, gl, y);
-    // What lies behind the row's end may be anything, and a 0 in dz does not make up for it.
-    constexpr int kPart = S::kShifted ? 1 : S::VEC / 2;   // pairs that are there or not together, but for a ragged end
+    // What lies behind the row's end may be anything, and a 0 in dz does not make up for it: a last piece that is not full is
+    // cleared here, and pieces that no lane copies hold the zeros the kernel began with.
+    if (ragged) {
 #pragma unroll
-    for (int c = 0; c < S::kPairs; c += kPart) {
-      if (2 * c / kVec * kApart >= left) continue;
-#pragma unroll
-      for (int i = c; i < c + kPart; ++i) {
-        if (ragged) {
-          const int k = 2 * i / kVec * kApart + 2 * i % kVec, k1 = (2 * i + 1) / kVec * kApart + (2 * i + 1) % kVec;
-          const float2 p = as_floats(y[i]);
-          y[i] = as_pair(k < left ? __float_as_uint(p.x) : 0u, k1 < left ? __float_as_uint(p.y) : 0u);
-        }
-        s = fma_pair(dz[i], y[i], s);
+      for (int i = 0; i < S::kPairs; ++i) {
+        const int k = 2 * i / kVec * kApart + 2 * i % kVec, k1 = (2 * i + 1) / kVec * kApart + (2 * i + 1) % kVec;
+        const float2 p = as_floats(y[i]);
+        y[i] = as_pair(k < left ? __float_as_uint(p.x) : 0u, k1 < left ? __float_as_uint(p.y) : 0u);
       }
     }
+    uint64_t t = 0;   // two chains
+#pragma unroll
+    for (int i = 0; i < S::kPairs; i += 2) {
+      s = fma_pair(dz[i], y[i], s);
+      t = fma_pair(dz[i + 1], y[i + 1], t);
+    }
+    s = add_pair(s, t);
     dot[used++ % kAtOnce] = as_floats(s).x + as_floats(s).y;
   }
   __device__ __forceinline__ void steps_done(int place, bool in) {
@@ -187,7 +200,7 @@ struct GradWork {
 };
 
 template <int DT, int G, int CH>
-__global__ void __launch_bounds__(kWalkThreads, 640 / kWalkThreads)
+__global__ void __launch_bounds__(kWalkThreads, 512 / kWalkThreads)   // dy, z and dz of a row at a time
 value_grad_kernel(const __grid_constant__ ValueGradArgs a) {
   using S = Share<DT, G, CH>;
   extern __shared__ __align__(16) unsigned char grad_smem[];
@@ -197,8 +210,11 @@ value_grad_kernel(const __grid_constant__ ValueGradArgs a) {
   ptr.init(a.indptr, a.rows, a.nnz);
   const int64_t q = (int64_t)blockIdx.x * (kWalkThreads / 32) + w;
   if ((q << a.lg) >= ptr.total) return;
+  uint4* ring = reinterpret_cast<uint4*>(reinterpret_cast<WalkSmem*>(grad_smem)[w].ring);
+  for (int i = lane; i < kRingBytes / 16 + 1; i += 32) ring[i] = make_uint4(0u, 0u, 0u, 0u);
+  __syncwarp();
   const WalkArgs wa{a.indices + ptr.base, nullptr, nullptr, nullptr, reinterpret_cast<const char*>(a.B) + (int64_t)a.f0 * dtype_bytes(DT), a.pitch_b, nf};
-  GradWork<DT, G, CH> work{a, a.f0 + first, nf - first, lane % G, S::kShifted || a.N % S::VEC != 0};
+  GradWork<DT, G, CH> work{a, a.f0 + first, nf - first, lane % G, S::kShifted || a.N % S::VEC != 0, !S::kShifted && a.vec && a.N % S::VEC == 0};
   RowWalk<DT, G, CH, false, GradWork<DT, G, CH>>(wa, ptr, reinterpret_cast<WalkSmem*>(grad_smem)[w], work).range(q, a.lg, a.slack);
 }
 
@@ -283,7 +299,8 @@ int lf_spmm_csr_grad_values(const int64_t* indptr, const int32_t* indices, int64
   const uint32_t bytes = (uint32_t)dtype_bytes(dy_dtype);
   const ValueGradArgs a{indptr + row_begin, indices, nnz, dy, activation == LF_ACT_NONE ? nullptr : preact, B, dvalues,
                         (uint32_t)ld_dy * bytes, (uint32_t)ld_preact * bytes, (uint32_t)ldb * dtype_bytes(b_dtype),
-                        (int)(row_end - row_begin), N, dy_dtype, activation, lg, range_slack(lg), 0};
+                        (int)(row_end - row_begin), N, dy_dtype, activation, lg, range_slack(lg), 0,
+                        on_grid16(dy, ld_dy, dy_dtype) && (activation == LF_ACT_NONE || on_grid16(preact, ld_preact, dy_dtype))};
   cudaStream_t st = (cudaStream_t)stream;
   if (b_dtype == LF_DTYPE_F32) LF_CUDA_CHECK(launch_value_grad<LF_DTYPE_F32>(a, st));
   else if (b_dtype == LF_DTYPE_BF16) LF_CUDA_CHECK(launch_value_grad<LF_DTYPE_BF16>(a, st));
