@@ -126,7 +126,9 @@ __device__ __forceinline__ void finish8(const ActArgs& a, int row, int f, const 
 }
 
 // ---- the walk ---------------------------------------------------------------------------------------
-template <int DT, int G, int CH>
+// VIO: rows of C, residual and preact are known to be on the grid.  Only the 8-bit form is compiled for that (2^20 uniform
+// rows of 64 features 790 -> 724 us, the shorter code); the 16-bit one is slower so (2^20 power-law rows 624 -> 687).
+template <int DT, int G, int CH, bool VIO>
 struct ActWork {
   using S = Share<DT, G, CH>;
   // the lane's share of a row in memory
@@ -136,7 +138,7 @@ struct ActWork {
   const float* bias;    // in shared memory, from the lane's first feature on
   int64_t slots;        // of the range in `partial`
   int f, left, gl;      // the lane's first feature; features from there to the end of the walk
-  bool vec;
+  bool vec_;
   uint64_t sum[S::kPairs];
   __align__(16) uint32_t res[S::kFloats];
 
@@ -146,11 +148,12 @@ struct ActWork {
     for (int i = 0; i < (int)(a.N * dtype_bytes(a.res_dtype)); i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + i));
   }
   static constexpr bool kPlaces = false;
+  __device__ __forceinline__ bool vec() const { return VIO || vec_; }
   __device__ __forceinline__ void begin(int row, bool whole, int piece, int64_t, int) {
 #pragma unroll
     for (int i = 0; i < S::kPairs; ++i) sum[i] = 0;
     if (a.residual && row >= 0 && !(whole && piece >= 0))   // on its way while the row is summed up
-      Io::load(row_at(a.residual, row, a.pitch_res) + f * dtype_bytes(a.res_dtype), a.res_dtype, vec, kApart, left, res);
+      Io::load(row_at(a.residual, row, a.pitch_res) + f * dtype_bytes(a.res_dtype), a.res_dtype, vec(), kApart, left, res);
   }
   __device__ __forceinline__ void step(float v, const unsigned char* x) {
     uint64_t y[S::kPairs];
@@ -183,12 +186,12 @@ struct ActWork {
       for (int i = 0; i < S::kFloats; ++i)
         if (i / kBlock * kApart + i % kBlock < left) p[i / kBlock * kApart + i % kBlock] = z[i];
     } else {
-      Io::finish(a, vec, row, f, kApart, left, bias, res, z);
+      Io::finish(a, vec(), row, f, kApart, left, bias, res, z);
     }
   }
 };
 
-template <int DT, int G, int CH, bool IND>
+template <int DT, int G, int CH, bool IND, bool VIO>
 __global__ void __launch_bounds__(kWalkThreads, 640 / kWalkThreads)
 spmm_csr_act_kernel(const __grid_constant__ ActArgs a) {
   using S = Share<DT, G, CH>;
@@ -207,8 +210,8 @@ spmm_csr_act_kernel(const __grid_constant__ ActArgs a) {
   const WalkArgs wa{a.indices + ptr.base, a.data && !a.order ? a.data + ptr.base : a.data, a.order ? a.order + ptr.base : nullptr, a.b_scale,
                     reinterpret_cast<const char*>(a.B) + (int64_t)f0 * dtype_bytes(DT), a.pitch_b, nf};
   const int first = S::feature(0, lane % G);
-  ActWork<DT, G, CH> work{a, bias + first, 2 * q, f0 + first, nf - first, lane % G, !S::kShifted && a.vec && a.N % ActWork<DT, G, CH>::kBlock == 0};
-  RowWalk<DT, G, CH, IND, ActWork<DT, G, CH>>(wa, ptr, walks[w], work).range(q, a.lg, a.slack);
+  ActWork<DT, G, CH, VIO> work{a, bias + first, 2 * q, f0 + first, nf - first, lane % G, !S::kShifted && a.vec && a.N % ActWork<DT, G, CH, VIO>::kBlock == 0};
+  RowWalk<DT, G, CH, IND, ActWork<DT, G, CH, VIO>>(wa, ptr, walks[w], work).range(q, a.lg, a.slack);
 }
 
 // Rows without entries, and rows that several ranges share: their pieces in order.  A lane has eight features; rows of few pieces
@@ -226,7 +229,7 @@ __device__ __forceinline__ void add_piece(const ActArgs& a, int64_t slot, int f,
   z[4] += y.x; z[5] += y.y; z[6] += y.z; z[7] += y.w;
 }
 
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 6)   // most blocks only look at row pointers: many of them at a time
 finish_rows_kernel(const __grid_constant__ ActArgs a, int span) {   // span: rows of a block at a time, at most its threads
   __shared__ int rows_of[kThreads / 32][32], long_rows[kThreads], num_long;
   __shared__ int64_t starts_of[kThreads / 32][32], ends_of[kThreads / 32][32];
@@ -306,10 +309,10 @@ finish_rows_kernel(const __grid_constant__ ActArgs a, int span) {   // span: row
   }
 }
 
-template <int DT, int G, int CH, bool IND>
+template <int DT, int G, int CH, bool IND, bool VIO>
 cudaError_t launch_walk_as(const ActArgs& a, cudaStream_t st) {
   using S = Share<DT, G, CH>;
-  constexpr auto kernel = spmm_csr_act_kernel<DT, G, CH, IND>;
+  constexpr auto kernel = spmm_csr_act_kernel<DT, G, CH, IND, VIO>;
   constexpr int smem = kWalkThreads / 32 * (int)sizeof(WalkSmem) + S::kSpan * 4;
   const cudaError_t e = allow_smem<kernel>(smem);
   if (e != cudaSuccess) return e;
@@ -321,9 +324,12 @@ cudaError_t launch_walk_as(const ActArgs& a, cudaStream_t st) {
 template <int DT>
 cudaError_t launch_walk(const ActArgs& a, cudaStream_t st) {
   return with_row_shape<DT>((uintptr_t)a.B % 16 == 0 && a.pitch_b % 16 == 0, a.N, [&](auto G, auto CH) {
-    if constexpr (DT != LF_DTYPE_E4M3)
-      if (!a.b_scale && !a.order) return launch_walk_as<DT, G.value, CH.value, false>(a, st);
-    return launch_walk_as<DT, G.value, CH.value, true>(a, st);
+    if constexpr (DT != LF_DTYPE_E4M3) {
+      if (!a.b_scale && !a.order) return launch_walk_as<DT, G.value, CH.value, false, false>(a, st);
+    } else if constexpr (CH.value > 0) {
+      if (a.vec && a.N % ActWork<DT, G.value, CH.value, true>::kBlock == 0) return launch_walk_as<DT, G.value, CH.value, true, true>(a, st);
+    }
+    return launch_walk_as<DT, G.value, CH.value, true, false>(a, st);
   });
 }
 

@@ -32,17 +32,19 @@ from .hyb import DeviceCsr, Workspace
 ACTIVATIONS = {None: _cabi.LF_ACT_NONE, "none": _cabi.LF_ACT_NONE, "relu": _cabi.LF_ACT_RELU, "silu": _cabi.LF_ACT_SILU,
                "gelu": _cabi.LF_ACT_GELU, "gelu_tanh": _cabi.LF_ACT_GELU_TANH}
 
-_codes = {}
+_wide, _any = {}, {}     # LF_DTYPE_* of torch's types: 16 and 32 bits, and with e4m3
 
 
-def _code(dtype, allowed="wide"):
-    """``LF_DTYPE_*`` of a torch type; ``allowed``: "wide" (16 and 32 bits) or "any" (e4m3 too)."""
-    if not _codes:
-        torch = _torch()
-        _codes.update({torch.float32: _cabi.LF_DTYPE_F32, torch.bfloat16: _cabi.LF_DTYPE_BF16,
-                       torch.float16: _cabi.LF_DTYPE_F16, torch.float8_e4m3fn: _cabi.LF_DTYPE_E4M3})
-    code = _codes.get(dtype)
-    if code is None or (allowed == "wide" and code == _cabi.LF_DTYPE_E4M3):
+def _code(dtype, codes=_wide):
+    """``LF_DTYPE_*`` of a torch type."""
+    code = codes.get(dtype)
+    if code is None:
+        if not _wide:
+            torch = _torch()
+            _wide.update({torch.float32: _cabi.LF_DTYPE_F32, torch.bfloat16: _cabi.LF_DTYPE_BF16, torch.float16: _cabi.LF_DTYPE_F16})
+            _any.update(_wide)
+            _any[torch.float8_e4m3fn] = _cabi.LF_DTYPE_E4M3
+            return _code(dtype, codes)
         raise ValueError(f"type {dtype} is not supported here")
     return code
 
@@ -92,6 +94,17 @@ def _act_code(activation):
     return code
 
 
+def _run(fn, call, dev):
+    """``fn(*call)`` with ``dev`` current (a guard costs more than the rest of a small call)."""
+    if _torch()._C._cuda_getDevice() == dev:
+        status = fn(*call)
+    else:
+        with on_device(dev):
+            status = fn(*call)
+    if status:
+        check(status)
+
+
 def _scratch(nbytes, workspace, device):
     if nbytes == 0:
         return None, 0
@@ -131,7 +144,7 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, out_dtype=None, out=No
     w_code = _code(weight.dtype)
     if out_dtype is None:
         out_dtype = x.dtype if out is None else out.dtype
-    y_code = _code(out_dtype, "any")
+    y_code = _code(out_dtype, _any)
     e4m3 = y_code == _cabi.LF_DTYPE_E4M3
     if out is None:
         out = empty_rows(M, N, out_dtype, x.device) if e4m3 else torch.empty((M, N), dtype=out_dtype, device=x.device)
@@ -154,9 +167,9 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, out_dtype=None, out=No
         rstd = torch.empty(M, dtype=torch.float32, device=x.device)
     s_ptr = _vector(scale, "scale", M, dev, torch.float32) if e4m3 else 0
     r_ptr = _vector(rstd, "rstd", M, dev, torch.float32)
-    with on_device(dev):
-        check(_cabi.load().lf_rms_norm(x.data_ptr(), code, ld_x, res_ptr, ld_res, sum_ptr, ld_sum, w, w_code, float(eps),
-                                       out.data_ptr(), y_code, ld_y, s_ptr, r_ptr, M, N, stream_of(dev)))
+    call = (x.data_ptr(), code, ld_x, res_ptr, ld_res, sum_ptr, ld_sum, w, w_code, eps, out.data_ptr(), y_code, ld_y, s_ptr,
+            r_ptr, M, N, stream_of(dev))
+    _run(_cabi.load().lf_rms_norm, call, dev)
     return NormOutput(out, scale, h, rstd)
 
 
@@ -181,11 +194,10 @@ def rms_norm_backward(dy, h, weight, rstd, dh=None, dx=None, dweight=None, works
     w, w_code, r = _vector(weight, "weight", N, dev), _code(weight.dtype), _vector(rstd, "rstd", M, dev, torch.float32)
     dw = _vector(dweight, "dweight", N, dev, torch.float32)
     nbytes = lib.lf_rms_norm_backward_workspace_bytes(M, N)
-    with on_device(dev):
-        keep, ws = _scratch(nbytes, workspace, dy.device)
-        check(lib.lf_rms_norm_backward(dy.data_ptr(), ld_dy, h.data_ptr(), ld_h, code, w, w_code, r,
-                                       0 if dh is None else dh.data_ptr(), ld_dh, dx.data_ptr(), ld_dx, dw, M, N, ws, nbytes,
-                                       stream_of(dev)))
+    keep, ws = _scratch(nbytes, workspace, dy.device)
+    call = (dy.data_ptr(), ld_dy, h.data_ptr(), ld_h, code, w, w_code, r, 0 if dh is None else dh.data_ptr(), ld_dh,
+            dx.data_ptr(), ld_dx, dw, M, N, ws, nbytes, stream_of(dev))
+    _run(lib.lf_rms_norm_backward, call, dev)
     return dx, dweight
 
 
@@ -223,13 +235,6 @@ class CsrTranspose:
         return CsrTranspose.from_host(csr.indptr.cpu().numpy(), csr.indices.cpu().numpy(), csr.shape, csr.indptr.device)
 
 
-def _product(lib, a, data, order, r0, r1, nnz, B, b_code, ldb, scale_ptr, out, ldc, N, ep, workspace, dev):
-    nbytes = lib.lf_spmm_csr_act_workspace_bytes(nnz, N, b_code)
-    keep, ws = _scratch(nbytes, workspace, B.device)
-    check(lib.lf_spmm_csr_act(a.indptr.data_ptr(), a.indices.data_ptr(), data, order, r0, r1, nnz, B.data_ptr(), b_code, ldb,
-                              scale_ptr, out.data_ptr(), _code(out.dtype), ldc, N, ep, ws, nbytes, stream_of(dev)))
-
-
 def _csr_arrays(a, values, dev):
     """Addresses of the values and of their order."""
     transposed = isinstance(a, CsrTranspose)
@@ -258,7 +263,7 @@ def spmm_csr_act(a, B, scale=None, bias=None, activation: Optional[str] = None, 
     lib = _cabi.load()
     K, N, dev = _first(B, "B")
     _need(K == a.shape[1], "B must have one row per matrix column")
-    b_code = _code(B.dtype, "any")
+    b_code = _code(B.dtype, _any)
     ldb = _matrix(B, "B", K, N, dev)
     act = _act_code(activation)
     _need(b_code != _cabi.LF_DTYPE_E4M3 or scale is not None, "8-bit rows need their scales")
@@ -275,21 +280,23 @@ def spmm_csr_act(a, B, scale=None, bias=None, activation: Optional[str] = None, 
         out = torch.empty((r1 - r0, N), dtype=out_dtype, device=B.device)
     _need(out.dtype == out_dtype, "out must have out_dtype")
     ldc = _matrix(out, "out", r1 - r0, N, dev)
-    ep = LfEpilogue()
-    ep.activation = act
+    c_ptr = out.data_ptr()
+    b_ptr = b_type = r_ptr = r_type = ld_res = z_ptr = ld_z = 0
     if bias is not None:
-        ep.bias, ep.bias_dtype = _vector(bias, "bias", N, dev), _code(bias.dtype)
+        b_ptr, b_type = _vector(bias, "bias", N, dev), _code(bias.dtype)
     if residual is not None:
-        ep.ld_residual = _matrix(residual, "residual", r1 - r0, N, dev)
-        ep.residual, ep.residual_dtype = residual.data_ptr(), _code(residual.dtype)
-        _need(residual.data_ptr() != out.data_ptr() or (residual.dtype == out_dtype and ep.ld_residual == ldc),
-              "a residual at out's address must be out")
+        r_ptr, r_type, ld_res = residual.data_ptr(), _code(residual.dtype), _matrix(residual, "residual", r1 - r0, N, dev)
+        _need(r_ptr != c_ptr or (residual.dtype == out_dtype and ld_res == ldc), "a residual at out's address must be out")
     if preact is not None:
         _need(preact.dtype == out_dtype, "preact must have the result's type")
-        ep.preact, ep.ld_preact = preact.data_ptr(), _matrix(preact, "preact", r1 - r0, N, dev)
+        z_ptr, ld_z = preact.data_ptr(), _matrix(preact, "preact", r1 - r0, N, dev)
+    ep = LfEpilogue(b_ptr, r_ptr, z_ptr, ld_res, ld_z, b_type, r_type, act)
     s_ptr = 0 if scale is None else _vector(scale, "scale", K, dev, torch.float32)
-    with on_device(dev):
-        _product(lib, a, data, order, r0, r1, nnz, B, b_code, ldb, s_ptr, out, ldc, N, C.byref(ep), workspace, dev)
+    nbytes = lib.lf_spmm_csr_act_workspace_bytes(nnz, N, b_code)
+    keep, ws = _scratch(nbytes, workspace, B.device)
+    call = (a.indptr.data_ptr(), a.indices.data_ptr(), data, order, r0, r1, nnz, B.data_ptr(), b_code, ldb, s_ptr, c_ptr,
+            _code(out_dtype), ldc, N, C.byref(ep), ws, nbytes, stream_of(dev))
+    _run(lib.lf_spmm_csr_act, call, dev)
     return out
 
 
@@ -314,10 +321,10 @@ def act_backward(dy, preact=None, activation: Optional[str] = None, dz=None, nee
     ld_dz = 0 if dz is None else _matrix(dz, "dz", M, N, dev)
     b_ptr = 0 if dbias is None else _vector(dbias, "dbias", N, dev, torch.float32)
     nbytes = 0 if dbias is None else lib.lf_act_backward_workspace_bytes(M, N)
-    with on_device(dev):
-        keep, ws = _scratch(nbytes, workspace, dy.device)
-        check(lib.lf_act_backward(dy.data_ptr(), ld_dy, 0 if act == _cabi.LF_ACT_NONE else preact.data_ptr(), ld_z, code, act,
-                                  0 if dz is None else dz.data_ptr(), ld_dz, b_ptr, M, N, ws, nbytes, stream_of(dev)))
+    keep, ws = _scratch(nbytes, workspace, dy.device)
+    call = (dy.data_ptr(), ld_dy, 0 if act == _cabi.LF_ACT_NONE else preact.data_ptr(), ld_z, code, act,
+            0 if dz is None else dz.data_ptr(), ld_dz, b_ptr, M, N, ws, nbytes, stream_of(dev))
+    _run(lib.lf_act_backward, call, dev)
     return dz, dbias
 
 
@@ -337,11 +344,10 @@ def spmm_csr_grad_values(a: DeviceCsr, B, dy, preact=None, activation: Optional[
     if out is None:
         out = torch.empty(a.nnz, dtype=torch.float32, device=B.device)
     o_ptr = _vector(out, "out", a.nnz, dev, torch.float32)
-    with on_device(dev):
-        check(_cabi.load().lf_spmm_csr_grad_values(
-            a.indptr.data_ptr(), a.indices.data_ptr(), 0, M, a.nnz, dy.data_ptr(), ld_dy,
+    call = (a.indptr.data_ptr(), a.indices.data_ptr(), 0, M, a.nnz, dy.data_ptr(), ld_dy,
             0 if act == _cabi.LF_ACT_NONE else preact.data_ptr(), ld_z, _code(dy.dtype), act, B.data_ptr(), _code(B.dtype), ldb,
-            N, o_ptr, stream_of(dev)))
+            N, o_ptr, stream_of(dev))
+    _run(_cabi.load().lf_spmm_csr_grad_values, call, dev)
     return out
 
 
