@@ -446,9 +446,9 @@ typedef struct lf_epilogue {
  * B, or NULL for any type but e4m3); C float32, bfloat16 or float16.  order (or NULL): entry e takes
  * data[order[e]] -- A transposed, given by its own indptr and indices, over the values of A.  An
  * entry whose value is 0 reads nothing of B (nor its scale), so it passes on no NaN or infinity.
- * nnz: the exact number of entries of the rows.  The workspace holds the sums of rows that several
+ * nnz: the exact number of entries of the rows, for the workspace's size too (it does not grow steadily).  The workspace holds the sums of rows that several
  * thread groups share; it may be used again as soon as the call is over on the stream, not by two
- * calls at a time.  Fewer than 2^31 rows, ldb and ldc below 2^30.  Rows of B off the 16-byte grid are read in
+ * calls at a time.  Fewer than 2^31 rows, every stride below 2^30, at most 2^22 features.  Rows of B off the 16-byte grid are read in
  * the aligned 16-byte pieces that cover them, as in lf_spmm_csr_f32. */
 size_t lf_spmm_csr_act_workspace_bytes(int64_t nnz, int32_t N, int32_t b_dtype);
 int lf_spmm_csr_act(const int64_t* indptr /*[dev]*/, const int32_t* indices /*[dev]*/,
@@ -467,8 +467,8 @@ int lf_act_backward(const void* dy /*[dev]*/, int64_t ld_dy, const void* preact 
                     size_t workspace_bytes, void* stream);
 
 /* Gradient of the values: dvalues[e] = <dy[r,:] * activation'(preact[r,:]), B[indices[e],:]> for the
- * entries e of the rows r of [row_begin, row_end), counted from the first of them; dy and preact start at
- * row row_begin and have dy_dtype. */
+ * entries e of the rows r of [row_begin, row_end), those of value 0 among them, counted from the first; dy and
+ * preact start at row row_begin and have dy_dtype.  Rows, strides and features as for lf_spmm_csr_act. */
 int lf_spmm_csr_grad_values(const int64_t* indptr /*[dev]*/, const int32_t* indices /*[dev]*/, int64_t row_begin,
                             int64_t row_end, int64_t nnz, const void* dy /*[dev]*/, int64_t ld_dy,
                             const void* preact /*[dev]*/, int64_t ld_preact, int32_t dy_dtype, int32_t activation,

@@ -3,7 +3,7 @@
 //
 // A warp is R = 32 / G groups of G lanes; a row of B is CH pieces of 16 bytes per lane of a group.  The warp takes up to 32
 // consecutive rows at a time, brings their columns and values into shared memory, sorts the rows by length and does R of
-// them side by side, a group each; rows of more than 32 entries are done by all groups together.  Either way the rows of
+// them side by side, a group each; rows of more than 64 entries are done by all groups together.  Either way the rows of
 // B come through a ring in shared memory that cp.async fills 8 KB ahead, across the rows' ends.
 //
 // Why sorted rows: graphs have most of their rows at a few entries and most of their entries in a few rows.  Groups that
@@ -236,7 +236,7 @@ struct WalkArgs {
 
 constexpr int kWalkThreads = 64;    // two warps: a block ends with the slower of two ranges (four: 3 % more on the graph above)
 constexpr int kWindow = 256;        // entries of the rows taken at a time, rows rounded up to fours
-constexpr int kShortRow = 32;       // longest row that one group does
+constexpr int kShortRow = 64;       // longest row that one group does (16 / 32 / 64 / 128: 713 / 622 / 606 / 642 us on the graph above)
 constexpr int kAtOnce = 4;          // steps (a row of B per group) that are copied and added up together
 constexpr int kRingBytes = 8192;
 constexpr uint32_t kNothing = 0x80000000u;   // mark of a column whose row of B is not read

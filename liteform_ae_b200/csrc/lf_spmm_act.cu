@@ -137,6 +137,7 @@ struct ActWork {
   const ActArgs& a;
   const float* bias;    // in shared memory, from the lane's first feature on
   int64_t slots;        // of the range in `partial`
+  int f0, nf;           // the walk's features
   int f, left, gl;      // the lane's first feature; features from there to the end of the walk
   bool vec_;
   uint64_t sum[S::kPairs];
@@ -144,8 +145,9 @@ struct ActWork {
 
   __device__ __forceinline__ void coming(int row) const {   // the residual, 128 bytes at a time
     if (!a.residual) return;
-    const char* p = row_at(a.residual, row, a.pitch_res);
-    for (int i = 0; i < (int)(a.N * dtype_bytes(a.res_dtype)); i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + i));
+    const int bytes = dtype_bytes(a.res_dtype);
+    const char* p = row_at(a.residual, row, a.pitch_res) + f0 * bytes;
+    for (int i = 0; i < nf * bytes; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + i));
   }
   static constexpr bool kPlaces = false;
   __device__ __forceinline__ bool vec() const { return VIO || vec_; }
@@ -210,7 +212,7 @@ spmm_csr_act_kernel(const __grid_constant__ ActArgs a) {
   const WalkArgs wa{a.indices + ptr.base, a.data && !a.order ? a.data + ptr.base : a.data, a.order ? a.order + ptr.base : nullptr, a.b_scale,
                     reinterpret_cast<const char*>(a.B) + (int64_t)f0 * dtype_bytes(DT), a.pitch_b, nf};
   const int first = S::feature(0, lane % G);
-  ActWork<DT, G, CH, VIO> work{a, bias + first, 2 * q, f0 + first, nf - first, lane % G, !S::kShifted && a.vec && a.N % ActWork<DT, G, CH, VIO>::kBlock == 0};
+  ActWork<DT, G, CH, VIO> work{a, bias + first, 2 * q, f0, nf, f0 + first, nf - first, lane % G, !S::kShifted && a.vec && a.N % ActWork<DT, G, CH, VIO>::kBlock == 0};
   RowWalk<DT, G, CH, IND, ActWork<DT, G, CH, VIO>>(wa, ptr, walks[w], work).range(q, a.lg, a.slack);
 }
 
@@ -350,6 +352,7 @@ int lf_spmm_csr_act(const int64_t* indptr, const int32_t* indices, const float* 
                     const float* b_scale, void* C, int32_t c_dtype, int64_t ldc, int32_t N, const lf_epilogue* epilogue,
                     void* workspace, size_t workspace_bytes, void* stream) {
   LF_REQUIRE(N >= 1 && ldb >= N && ldc >= N && ldb < (1ll << 30) && ldc < (1ll << 30), "bad sizes");
+  LF_REQUIRE(N <= (1 << 22), "more than 2^22 features");
   LF_REQUIRE(0 <= row_begin && row_begin <= row_end, "bad row range");
   LF_REQUIRE(row_end - row_begin < (1ll << 31) - 64 && nnz >= 0, "bad number of rows or entries");
   LF_REQUIRE(b_dtype == LF_DTYPE_E4M3 || is_wide_dtype(b_dtype), "unknown type of B");

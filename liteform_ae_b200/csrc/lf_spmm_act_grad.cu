@@ -93,7 +93,7 @@ struct GradWork {
   static constexpr bool kPlaces = true;
   static constexpr int kVec = S::kShifted ? 1 : S::VEC, kApart = S::kShifted ? G : G * S::VEC;
   const ValueGradArgs& a;
-  int f, left, gl;
+  int f0, nf, f, left, gl;   // the walk's features; the lane's first, and those from there on
   bool ragged, vec;        // the row's last piece of 16 bytes is not full; rows of dy and z are on the 16-byte grid
   int stop, used;
   int64_t at;
@@ -105,8 +105,9 @@ struct GradWork {
     if (a.z) prefetch(a.z, row, a.pitch_z);
   }
   __device__ __forceinline__ void prefetch(const void* base, int row, uint32_t pitch) const {
-    const char* p = reinterpret_cast<const char*>(row_of_b(base, (uint32_t)row, pitch));
-    for (int i = 0; i < a.N * dtype_bytes(a.dy_dtype); i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + i));
+    const int bytes = dtype_bytes(a.dy_dtype);
+    const char* p = reinterpret_cast<const char*>(row_of_b(base, (uint32_t)row, pitch)) + f0 * bytes;
+    for (int i = 0; i < nf * bytes; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + i));
   }
   // the lane's features of a row, as floats; what lies behind its end is anything
   __device__ __forceinline__ void load(const void* base, int row, uint32_t pitch, float* v) const {
@@ -214,7 +215,7 @@ value_grad_kernel(const __grid_constant__ ValueGradArgs a) {
   for (int i = lane; i < kRingBytes / 16 + 1; i += 32) ring[i] = make_uint4(0u, 0u, 0u, 0u);
   __syncwarp();
   const WalkArgs wa{a.indices + ptr.base, nullptr, nullptr, nullptr, reinterpret_cast<const char*>(a.B) + (int64_t)a.f0 * dtype_bytes(DT), a.pitch_b, nf};
-  GradWork<DT, G, CH> work{a, a.f0 + first, nf - first, lane % G, S::kShifted || a.N % S::VEC != 0, !S::kShifted && a.vec && a.N % S::VEC == 0};
+  GradWork<DT, G, CH> work{a, a.f0, nf, a.f0 + first, nf - first, lane % G, S::kShifted || a.N % S::VEC != 0, !S::kShifted && a.vec && a.N % S::VEC == 0};
   RowWalk<DT, G, CH, false, GradWork<DT, G, CH>>(wa, ptr, reinterpret_cast<WalkSmem*>(grad_smem)[w], work).range(q, a.lg, a.slack);
 }
 
@@ -287,7 +288,7 @@ int lf_spmm_csr_grad_values(const int64_t* indptr, const int32_t* indices, int64
                             int64_t nnz, const void* dy, int64_t ld_dy, const void* preact, int64_t ld_preact,
                             int32_t dy_dtype, int32_t activation, const void* B, int32_t b_dtype, int64_t ldb,
                             int32_t N, float* dvalues, void* stream) {
-  LF_REQUIRE(N >= 1 && ldb >= N && ldb < (1ll << 30) && ld_dy >= N && ld_dy < (1ll << 30), "bad sizes");
+  LF_REQUIRE(N >= 1 && N <= (1 << 22) && ldb >= N && ldb < (1ll << 30) && ld_dy >= N && ld_dy < (1ll << 30), "bad sizes");
   LF_REQUIRE(0 <= row_begin && row_begin <= row_end && row_end - row_begin < (1ll << 31) - 64 && nnz >= 0, "bad row range");
   LF_REQUIRE(is_wide_dtype(dy_dtype) && is_wide_dtype(b_dtype), "the types must be float32, bfloat16 or float16");
   LF_REQUIRE(activation >= LF_ACT_NONE && activation <= LF_ACT_GELU_TANH, "unknown activation");

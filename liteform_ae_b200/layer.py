@@ -105,11 +105,17 @@ def _run(fn, call, dev):
         check(status)
 
 
-def _scratch(nbytes, workspace, device):
+def _scratch(nbytes, workspace, like):
+    """``(buffer, address, size)`` of ``nbytes`` on the device of ``like``; the buffer has to outlive the call."""
     if nbytes == 0:
-        return None, 0
-    buf = _torch().empty(nbytes, dtype=_torch().uint8, device=device) if workspace is None else workspace.get(nbytes)
-    return buf, buf.data_ptr()
+        return None, 0, 0
+    torch = _torch()
+    if workspace is None:
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    else:
+        buf = workspace.get(nbytes)
+        _need(buf.get_device() == like.get_device(), "the workspace must be on the device of the operands")
+    return buf, buf.data_ptr(), buf.numel()
 
 
 def empty_rows(rows: int, N: int, dtype, device):
@@ -194,9 +200,9 @@ def rms_norm_backward(dy, h, weight, rstd, dh=None, dx=None, dweight=None, works
     w, w_code, r = _vector(weight, "weight", N, dev), _code(weight.dtype), _vector(rstd, "rstd", M, dev, torch.float32)
     dw = _vector(dweight, "dweight", N, dev, torch.float32)
     nbytes = lib.lf_rms_norm_backward_workspace_bytes(M, N)
-    keep, ws = _scratch(nbytes, workspace, dy.device)
+    keep, ws, nws = _scratch(nbytes, workspace, dy)
     call = (dy.data_ptr(), ld_dy, h.data_ptr(), ld_h, code, w, w_code, r, 0 if dh is None else dh.data_ptr(), ld_dh,
-            dx.data_ptr(), ld_dx, dw, M, N, ws, nbytes, stream_of(dev))
+            dx.data_ptr(), ld_dx, dw, M, N, ws, nws, stream_of(dev))
     _run(lib.lf_rms_norm_backward, call, dev)
     return dx, dweight
 
@@ -293,9 +299,9 @@ def spmm_csr_act(a, B, scale=None, bias=None, activation: Optional[str] = None, 
     ep = LfEpilogue(b_ptr, r_ptr, z_ptr, ld_res, ld_z, b_type, r_type, act)
     s_ptr = 0 if scale is None else _vector(scale, "scale", K, dev, torch.float32)
     nbytes = lib.lf_spmm_csr_act_workspace_bytes(nnz, N, b_code)
-    keep, ws = _scratch(nbytes, workspace, B.device)
+    keep, ws, nws = _scratch(nbytes, workspace, B)
     call = (a.indptr.data_ptr(), a.indices.data_ptr(), data, order, r0, r1, nnz, B.data_ptr(), b_code, ldb, s_ptr, c_ptr,
-            _code(out_dtype), ldc, N, C.byref(ep), ws, nbytes, stream_of(dev))
+            _code(out_dtype), ldc, N, C.byref(ep), ws, nws, stream_of(dev))
     _run(lib.lf_spmm_csr_act, call, dev)
     return out
 
@@ -321,9 +327,9 @@ def act_backward(dy, preact=None, activation: Optional[str] = None, dz=None, nee
     ld_dz = 0 if dz is None else _matrix(dz, "dz", M, N, dev)
     b_ptr = 0 if dbias is None else _vector(dbias, "dbias", N, dev, torch.float32)
     nbytes = 0 if dbias is None else lib.lf_act_backward_workspace_bytes(M, N)
-    keep, ws = _scratch(nbytes, workspace, dy.device)
+    keep, ws, nws = _scratch(nbytes, workspace, dy)
     call = (dy.data_ptr(), ld_dy, 0 if act == _cabi.LF_ACT_NONE else preact.data_ptr(), ld_z, code, act,
-            0 if dz is None else dz.data_ptr(), ld_dz, b_ptr, M, N, ws, nbytes, stream_of(dev))
+            0 if dz is None else dz.data_ptr(), ld_dz, b_ptr, M, N, ws, nws, stream_of(dev))
     _run(lib.lf_act_backward, call, dev)
     return dz, dbias
 

@@ -11,6 +11,9 @@ with the same decisions and the same column names, on this package's device path
 statistics from ``lf_row_stats``, width search / format / product from the composed-format
 entry points, blocks cut on the device, CSR product as the last resort.
 
+``infer`` is what the driver is for: the layers of a model on a matrix that it has loaded, each a norm, the
+product with the matrix and the end of the layer, with the rows between them kept in 8 bits.
+
 The two classifiers are scikit-learn models the reference ships as pickles; they are not part
 of this package.  Pass anything with a ``predict`` method (``joblib.load`` of the reference's
 files works); ``clf_partition=None`` falls back to this package's own chooser
@@ -26,6 +29,7 @@ from typing import Dict, Iterable, List, Optional, Sequence
 import numpy as np
 
 from . import format_algos as fa
+from . import hyb as _hyb
 from .format_matrix_market import MTX
 
 FORMAT_SELECTION_FEATURES = ["num_rows", "num_cols", "nnz", "avg_nnz_per_row", "min_nnz_per_row",
@@ -146,6 +150,34 @@ def run_matrix(g: MTX, clf_selection, clf_partition=None, feat_sizes: Iterable[i
             log(f"name: {g.name} format: {rec['format']} feat_size: {n} exe_time: {rec['time_exe_our(ms)']}")
         rows.append(rec)
     return rows
+
+
+def infer(g: MTX, x, layers: Sequence[dict], eight_bits: bool = True, eps: float = 1e-6, device="cuda"):
+    """``x`` (a matrix of 16- or 32-bit features, one row per column of the square matrix ``g``) through layers
+
+        h = h + y;   f = rms_norm(h) * norm;   y = activation(A @ f + bias)
+
+    starting from h = x and y = 0; returns the last h + y, in x's type.  A layer is a dict with ``norm`` (one weight
+    per feature) and optionally ``bias`` and ``activation`` (``layer.ACTIVATIONS``).  ``eight_bits``: the rows that
+    the product gathers are e4m3 with a scale each, a quarter of float32's bytes; otherwise x's type.  Nothing is
+    synchronised, and the matrix is uploaded once."""
+    import torch
+    from . import layer
+    csr = g.csr_device(device)
+    if csr.shape[0] != csr.shape[1]:
+        raise ValueError("the matrix must be square")
+    if not layers:
+        raise ValueError("no layers")
+    ws = _hyb.Workspace(csr.indptr.device)
+    y, h = None, x
+    for i, p in enumerate(layers):
+        n = layer.rms_norm(h if y is None else y, p["norm"], residual=None if y is None else h, eps=eps,
+                           out_dtype=torch.float8_e4m3fn if eight_bits else x.dtype)
+        h = n.h
+        last = i + 1 == len(layers)
+        y = layer.spmm_csr_act(csr, n.y, scale=n.scale, bias=p.get("bias"), activation=p.get("activation"),
+                               residual=h if last else None, out_dtype=x.dtype, workspace=ws)
+    return y
 
 
 def run(matrices: Sequence[MTX], clf_selection, clf_partition=None, **kwargs) -> Dict[str, list]:

@@ -57,13 +57,15 @@ def product(ep=None, **kw):
     return _cabi.load().lf_spmm_csr_act(*a.values(), 0)
 
 
-@pytest.mark.parametrize("kw", [dict(N=0), dict(ldb=7), dict(ldc=7), dict(ldb=1 << 30), dict(ldc=1 << 30), dict(r0=-1), dict(r0=3),
+@pytest.mark.parametrize("kw", [dict(N=0), dict(ldb=7), dict(ldc=7), dict(ldb=1 << 30), dict(ldc=1 << 30),
+                                dict(N=(1 << 22) + 1, ldb=1 << 23, ldc=1 << 23), dict(r0=-1), dict(r0=3),
                                 dict(r1=1 << 31), dict(nnz=-1), dict(bd=4), dict(cd=E4M3), dict(bd=E4M3), dict(indptr=0),
                                 dict(C=0), dict(indices=0), dict(B=0), dict(order=P, data=0), dict(order=P, nnz=1 << 31),
                                 dict(ep=dict(activation=5)), dict(ep=dict(activation=-1)), dict(ep=dict(bias=P, bias_dtype=E4M3)),
                                 dict(ep=dict(residual=P, residual_dtype=E4M3, ld_residual=8)),
                                 dict(ep=dict(residual=P, residual_dtype=F32, ld_residual=7)),
-                                dict(ep=dict(preact=P, ld_preact=7))])
+                                dict(ep=dict(preact=P, ld_preact=7)), dict(ep=dict(preact=P, ld_preact=1 << 30)),
+                                dict(ep=dict(residual=P, residual_dtype=F32, ld_residual=1 << 30))])
 def test_product_refusals(kw):
     assert product(**kw) == BAD
 
@@ -104,7 +106,8 @@ def value_grad(**kw):
     return _cabi.load().lf_spmm_csr_grad_values(*a.values(), 0)
 
 
-@pytest.mark.parametrize("kw", [dict(N=0), dict(ldb=7), dict(ldb=1 << 30), dict(ld_dy=7), dict(r0=3), dict(r0=-1), dict(nnz=-1),
+@pytest.mark.parametrize("kw", [dict(N=0), dict(N=(1 << 22) + 1, ldb=1 << 23, ld_dy=1 << 23, ld_z=1 << 23), dict(ldb=7),
+                                dict(ldb=1 << 30), dict(ld_dy=7), dict(ld_z=1 << 30), dict(r0=3), dict(r0=-1), dict(nnz=-1),
                                 dict(bd=E4M3), dict(dyd=E4M3), dict(act=9), dict(indptr=0), dict(indices=0), dict(dy=0), dict(B=0),
                                 dict(dv=0), dict(z=0), dict(ld_z=7)])
 def test_value_grad_refusals(kw):

@@ -614,3 +614,113 @@ def test_workspace_is_reused(cuda_device):
         assert torch.equal(layer.spmm_csr_act(A, B, workspace=ws), want)
         dz, db = layer.act_backward(want, want, "silu", workspace=ws)
         assert torch.equal(db, layer.act_backward(want, want, "silu")[1])
+
+
+def test_workspace_of_another_device_or_too_small(cuda_device):
+    class Small(hyb.Workspace):
+        def get(self, nbytes, slot=0):
+            return super().get(nbytes, slot)[:nbytes - 16]
+
+    p = pattern(20, 30, 1)
+    A = csr_on(cuda_device, p, (20, 30))
+    B = torch.randn(30, 16, device=cuda_device)
+    with pytest.raises(ValueError):
+        layer.spmm_csr_act(A, B, workspace=hyb.Workspace("cpu"))
+    with pytest.raises(_cabi.LiteformError):
+        layer.spmm_csr_act(A, B, workspace=Small(cuda_device))
+    with pytest.raises(_cabi.LiteformError):
+        layer.act_backward(B, workspace=Small(cuda_device))
+
+
+# ---- graphs large enough for every length of range, rows of many pieces, runs of empty rows ----------
+def big_pattern(M, K, entries, hubs, hub_len, used, seed, dev):
+    """CSR arrays on the device: `used` of the rows hold entries, `hubs` of them `hub_len`."""
+    g = torch.Generator(device=dev).manual_seed(seed)
+    where = torch.randperm(M, generator=g, device=dev)[:used]
+    r = where[torch.randint(0, used, (entries,), generator=g, device=dev)]
+    r = torch.cat([r] + [torch.full((hub_len,), int(h), device=dev) for h in where[:hubs]])
+    c = torch.randint(0, K, (r.numel(),), generator=g, device=dev)
+    keys = torch.unique(r * K + c)
+    rows = torch.div(keys, K, rounding_mode="floor")
+    indptr = torch.zeros(M + 1, dtype=torch.int64, device=dev)
+    torch.cumsum(torch.bincount(rows, minlength=M), 0, out=indptr[1:])
+    vals = torch.rand(keys.numel(), generator=g, device=dev) * 2 - 1
+    return rows, hyb.DeviceCsr(indptr, (keys - rows * K).int(), vals, (M, K))
+
+
+@pytest.mark.parametrize("M,K,entries,hubs,hub_len,used,N", [
+    (1 << 18, 1 << 17, 6_000_000, 3, 60_000, 1 << 18, 24),        # ranges of 1024 entries
+    (50_000, 90_000, 1_000_000, 20, 5000, 50_000, 40),            # 256
+    (300_000, 2000, 100, 0, 0, 60, 16),                           # nearly all rows empty
+    (3, 2_000_000, 10, 3, 900_000, 3, 8),                         # three rows of nearly a million entries
+    (200_000, 64, 30_000, 2, 60, 5, 33)])
+@pytest.mark.parametrize("dtype,out", [(F32, F32), (BF16, BF16), (E4M3, F16)])
+def test_large_graphs(cuda_device, M, K, entries, hubs, hub_len, used, N, dtype, out):
+    rows, A = big_pattern(M, K, entries, hubs, hub_len, used, M, cuda_device)
+    g = torch.Generator(device=cuda_device).manual_seed(N)
+    B = torch.randn((K, N), generator=g, device=cuda_device).to(dtype)
+    scale = torch.rand(K, generator=g, device=cuda_device) + 0.1 if dtype == E4M3 else None
+    Bv = B.double() * (1 if scale is None else scale.double()[:, None])
+    R = torch.randn((M, N), generator=g, device=cuda_device).to(out)
+    got = layer.spmm_csr_act(A, B, scale=scale, activation="relu", residual=R)  if dtype != E4M3 else \
+        layer.spmm_csr_act(A, B, scale=scale, activation="relu", residual=R, out_dtype=out)
+    full = lambda v, X: torch.sparse_csr_tensor(A.indptr, A.indices.long(), v, size=(M, K)) @ X
+    z, size = full(A.data.double(), Bv), full(A.data.double().abs(), Bv.abs())
+    n = torch.diff(A.indptr).double()[:, None]
+    y = z.clamp(min=0) + R.double()
+    off = (n + 3) * U32 * 1.01 * size + U32 * y.abs()
+    ref.close(got, y.cpu(), ref.rounded(y, off, out).cpu())
+    if dtype == E4M3:
+        return
+    dy = torch.randn((M, N), generator=g, device=cuda_device).to(dtype)
+    dv = layer.spmm_csr_grad_values(A, B, dy)
+    at = torch.randint(0, A.nnz, (min(A.nnz, 200_000),), generator=g, device=cuda_device)
+    prod = dy[rows[at]].double() * Bv[A.indices[at].long()]
+    ref.close(dv[at], prod.sum(1).cpu(), ((N + 3) * U32 * prod.abs().sum(1)).cpu(), "dvalues")
+    T = layer.CsrTranspose.of(A)
+    dB = layer.spmm_csr_act(T, dy, values=A.data, out_dtype=F32)
+    tr = lambda v, X: torch.sparse_csr_tensor(T.indptr, T.indices.long(), v[T.order.long()], size=(K, M)) @ X
+    want, size = tr(A.data.double(), dy.double()), tr(A.data.double().abs(), dy.double().abs())
+    n = torch.diff(T.indptr).double()[:, None]
+    ref.close(dB, want.cpu(), ((n + 3) * U32 * 1.01 * size + ref.TINY[F32]).cpu(), "dB")
+
+
+def test_values_of_other_numbers_than_the_matrix_has(cuda_device):
+    """nnz bounds what is read: a matrix whose row pointers promise more entries than there are stays inside them."""
+    indptr = torch.tensor([0, 4, 9, 40], device=cuda_device)
+    A = hyb.DeviceCsr(indptr, torch.arange(12, dtype=torch.int32, device=cuda_device), torch.ones(12, device=cuda_device), (3, 64))
+    B = torch.ones(64, 16, device=cuda_device)
+    y = layer.spmm_csr_act(A, B)
+    assert torch.equal(y[:, 0].cpu(), torch.tensor([4.0, 5.0, 3.0]))
+
+
+def test_infer(cuda_device):
+    """The pipeline's layers against the same steps, each from its own inputs, in 64 bits."""
+    from liteform_ae_b200 import pipeline, synth
+    from liteform_ae_b200.format_matrix_market import MTX
+    c = synth.zipf_rows(M=2048, seed=5)
+    m = MTX.from_csr(c.indptr, c.indices, c.data, c.shape, "t")
+    g, N = gen(3), 48
+    x = torch.randn(2048, N, generator=g).bfloat16().to(cuda_device)
+    layers = [dict(norm=(1 + 0.1 * torch.randn(N, generator=g)).to(cuda_device), bias=torch.randn(N, generator=g).to(cuda_device),
+                   activation="silu"), dict(norm=torch.ones(N, device=cuda_device), activation="gelu"),
+              dict(norm=torch.ones(N, device=cuda_device))]
+    A = m.csr_device(cuda_device)
+    for bits in (True, False):
+        got = pipeline.infer(m, x, layers, eight_bits=bits)
+        h, y = x, None
+        for i, p in enumerate(layers):
+            n = layer.rms_norm(h if y is None else y, p["norm"], residual=None if y is None else h, out_dtype=E4M3 if bits else BF16)
+            check_norm(h if y is None else y, None if y is None else h, None, 1e-6, n, (h if y is None else y).cpu().double(),
+                       None if y is None else h.cpu().double(), p["norm"].cpu().double())
+            f = n.y.cpu().double() * (n.scale.cpu().double()[:, None] if bits else 1)
+            a = ref.dense(A.indptr.cpu(), A.indices.cpu(), A.data.cpu(), A.shape)
+            h = n.h
+            _, want, _, off = ref.product(a, f, None if p.get("bias") is None else p["bias"].cpu(), p.get("activation") or "none",
+                                          h.cpu() if i == 2 else None, BF16)
+            y = layer.spmm_csr_act(A, n.y, scale=n.scale, bias=p.get("bias"), activation=p.get("activation"),
+                                   residual=h if i == 2 else None, out_dtype=BF16)
+            ref.close(y, want, off)
+        assert torch.equal(got, y)
+    with pytest.raises(ValueError):
+        pipeline.infer(m, x, [])
