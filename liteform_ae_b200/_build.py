@@ -5,11 +5,13 @@ back end and no fallback: a missing or stale library is an error at first use.
 """
 from __future__ import annotations
 
+import concurrent.futures
 import glob
 import os
 import shutil
 import subprocess
 import sys
+import tempfile
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _ROOT = os.path.dirname(_HERE)
@@ -63,15 +65,26 @@ def build_library(force: bool = False, verbose: bool = False, ptxas_info: bool =
     """(Re)build the shared library when a source is newer than it; returns its path."""
     if not force and not is_stale():
         return LIB_PATH
-    cmd = [find_nvcc()] + NVCC_FLAGS + (["-Xptxas", "-v"] if ptxas_info else []) + \
-        ["-o", LIB_PATH + ".tmp"] + SOURCES
-    if verbose:
-        print(" ".join(cmd), file=sys.stderr)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
-    if ptxas_info or verbose:
-        sys.stderr.write(res.stderr)
+    nvcc = find_nvcc()
+    flags = NVCC_FLAGS + (["-Xptxas", "-v"] if ptxas_info else [])
+
+    def run(cmd):
+        if verbose:
+            print(" ".join(cmd), file=sys.stderr)
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
+        if ptxas_info or verbose:
+            sys.stderr.write(res.stderr)
+
+    # one process per source, as many as there are processors, then the link (one after the other: 5.5 minutes)
+    with tempfile.TemporaryDirectory() as tmp:
+        objects = [os.path.join(tmp, os.path.basename(src)[:-3] + ".o") for src in SOURCES]
+        compile_flags = [f for f in flags if f != "-shared"]
+        with concurrent.futures.ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+            for done in [pool.submit(run, [nvcc] + compile_flags + ["-c", "-o", obj, src]) for src, obj in zip(SOURCES, objects)]:
+                done.result()
+        run([nvcc] + flags + ["-o", LIB_PATH + ".tmp"] + objects)
     os.replace(LIB_PATH + ".tmp", LIB_PATH)
     with open(BUILD_ID_PATH, "w") as f:
         f.write(source_id() + "\n")
