@@ -8,9 +8,10 @@
 //
 // Why sorted rows: graphs have most of their rows at a few entries and most of their entries in a few rows.  Groups that
 // end their rows at different steps run the epilogue one after the other; rows of about one length end together, and
-// nothing has to notice where a row ends.  2^20 power-law rows, 13.5 M entries, 128 bfloat16 features, bias, relu and
+// nothing has to notice where a row ends.  2^20 power-law rows, 13.2 M entries, 128 bfloat16 features, bias, relu and
 // residual: groups that walk over entries at an even pace, finished rows in a queue, 985 us; thread blocks that stage row
-// starts in the place of entries 1193; sorted rows with four gathers per group in registers instead of the ring 1441.
+// starts in the place of entries 1193; sorted rows with four gathers per group in registers instead of the ring 1441; as
+// it stands 620.
 #pragma once
 
 #include "lf_layer.cuh"
@@ -250,8 +251,7 @@ struct WalkSmem {
 
 // Copies the lane's pieces of a row of B into the ring (PIECES of 16 bytes, `STRIDE` apart in the row), those that are
 // `on`, or zeros for an entry that gathers nothing: the sums need not look, since what they multiply with its value 0 is 0.
-// Predicates and immediate offsets: with branches, addresses in registers and the number of bytes in one, a copy took 24 to
-// 50 instructions.
+// Predicates and immediate offsets, since this is a third of what the walk executes.
 template <int PIECES, int STRIDE, int TO>
 __device__ __forceinline__ void copy_row(uint32_t dst, const void* src, uint32_t col, int on1, int on2) {
   if constexpr (PIECES == 2) {

@@ -23,7 +23,8 @@ struct ActGradArgs {
 
 // A block's threads are 256 / per_row rows side by side, VEC features each; a thread keeps its features while it walks down
 // the rows, so that the bias's sum stays in registers.  The inputs are read once and dZ is written once: memory bounds it,
-// and, with the error function's slope, the instructions (2^18 rows of 256 bfloat16: see the table of measurements).
+// and, with the error function's slope, the special functions (2^18 rows of 256 bfloat16, gelu: 94 us, 4.3 TB/s; the bytes
+// alone would take 61).
 template <int DT, int VEC>
 __global__ void __launch_bounds__(256)
 act_grad_kernel(ActGradArgs a) {
@@ -86,7 +87,8 @@ struct ValueGradArgs {
 
 // The group keeps its row of dZ in registers (computed there, not rounded) and multiplies the rows of B that come through the
 // ring with it; four dot products at a time are summed up over the lanes, each lane ending with one of them.  A row wider
-// than a walk takes several launches, which add to what the ones before wrote.
+// than a walk takes several launches, which add to what the ones before wrote.  As in the product, the rows of B and the
+// instructions on them bound it (2^18 power-law rows, 3.1 M entries, 256 bfloat16 features, gelu: 455 us).
 template <int DT, int G, int CH>
 struct GradWork {
   using S = Share<DT, G, CH>;

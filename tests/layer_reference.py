@@ -37,12 +37,12 @@ def dense(indptr, indices, vals, shape):
     return a
 
 
-# Errors of the activations in 32 bits, absolute, for |z| as given: expf, __fdividef and erff are off by at most 2
-# units in the last place each (CUDA's tables), 1 + e and the products by half a unit; where the exponential's
-# argument is rounded (|t| 2^-24 relative in e^t, and |t| e^-t / (1 + e^-t) <= 0.28) or erf is near -1 the error is
-# absolute in what z is multiplied with.  16 units cover each form with room; the slopes add products of the same
-# terms with factors up to |z| (silu, gelu) and 1.6 |z| (1 + 0.134 z^2) where the sigmoid's complement is not 0
-# (the product of both stays below 3), for which 64 units are allowed.
+# Errors of the activations in 32 bits, absolute, for |z| as given: the special function unit's 2^x and 1 / x are off by
+# at most 2^-22 relative (4 units of 2^-24) and the series for the normal distribution by 7.5e-8 (1.3 units), 1 + e and
+# the products by half a unit; where the exponential's argument is rounded (|t| 2^-24 relative in e^t, and |t| e^-t / (1 +
+# e^-t) <= 0.28) or the distribution is near 1 the error is absolute in what z is multiplied with.  16 units cover each
+# form with room; the slopes add products of the same terms with factors up to |z| (silu, gelu) and 1.6 |z| (1 + 0.134 z^2)
+# where the sigmoid's complement is not 0 (the product of both stays below 3), for which 64 units are allowed.
 def act_error(z):
     return 16 * U[torch.float32] * z.abs()
 
