@@ -446,10 +446,12 @@ typedef struct lf_epilogue {
  * B, or NULL for any type but e4m3); C float32, bfloat16 or float16.  order (or NULL): entry e takes
  * data[order[e]] -- A transposed, given by its own indptr and indices, over the values of A.  An
  * entry whose value is 0 reads nothing of B (nor its scale), so it passes on no NaN or infinity.
- * nnz: the exact number of entries of the rows, for the workspace's size too (it does not grow steadily).  The workspace holds the sums of rows that several
- * thread groups share; it may be used again as soon as the call is over on the stream, not by two
- * calls at a time.  Fewer than 2^31 rows, every stride below 2^30, at most 2^22 features.  Rows of B off the 16-byte grid are read in
- * the aligned 16-byte pieces that cover them, as in lf_spmm_csr_f32. */
+ * nnz: the exact number of entries of the rows, for the workspace's size too (it does not grow
+ * steadily).  The workspace holds the sums of rows that several thread groups share; it may be used
+ * again as soon as the call is over on the stream, not by two calls at a time.  C and preact must not
+ * lie in B, nor in each other.  Fewer than 2^31 rows, every stride below 2^30, at most 2^22 features.
+ * Rows of B off the 16-byte grid are read in the aligned 16-byte pieces that cover them, as in
+ * lf_spmm_csr_f32. */
 size_t lf_spmm_csr_act_workspace_bytes(int64_t nnz, int32_t N, int32_t b_dtype);
 int lf_spmm_csr_act(const int64_t* indptr /*[dev]*/, const int32_t* indices /*[dev]*/,
                     const float* data /*[dev] or NULL: all ones*/, const int32_t* order /*[dev] or NULL*/,

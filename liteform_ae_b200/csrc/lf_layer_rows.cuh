@@ -11,7 +11,7 @@
 // nothing has to notice where a row ends.  2^20 power-law rows, 13.2 M entries, 128 bfloat16 features, bias, relu and
 // residual: groups that walk over entries at an even pace, finished rows in a queue, 985 us; thread blocks that stage row
 // starts in the place of entries 1193; sorted rows with four gathers per group in registers instead of the ring 1441; as
-// it stands 620.
+// it stands 563.
 #pragma once
 
 #include "lf_layer.cuh"
@@ -19,10 +19,11 @@
 
 namespace lf {
 
-// Entries of a warp's range: the most that still gives each of the chip's 148 SMs the 20 warps that it holds, three times
-// over where there are enough, from 64 to 1024.
+// Entries of a warp's range: the most that still gives each of the chip's 148 SMs the 20 warps that it could hold, three times
+// over where there are enough, from 64 to 2048 (2^20 uniform rows, 33.5 M entries: 735 us with 1024 each, 707 with 2048; the
+// power-law rows above 620 with 512, 615 with 1024).
 inline int range_log(int64_t nnz) {
-  int lg = 10;
+  int lg = 11;
   while (lg > 6 && (nnz >> lg) < 148 * 20 * (lg > 8 ? 3 : 1)) --lg;
   return lg;
 }
@@ -235,7 +236,8 @@ struct WalkArgs {
   int nf;                  // features from there on, at most kFeatures
 };
 
-constexpr int kWalkThreads = 64;    // two warps: a block ends with the slower of two ranges (four: 3 % more on the graph above)
+constexpr int kWalkThreads = 32;    // a warp: a block of two keeps its place until the slower is done (589 us on the graph above for 561)
+constexpr int kWalkBlocks = 17;     // per SM that the registers have to allow (shared memory: 19).  16: 614 us, 17: 563, 18: 560, 20: 585; the same in 8 bits: 712, 633, 642, 655
 constexpr int kWindow = 256;        // entries of the rows taken at a time, rows rounded up to fours
 constexpr int kShortRow = 64;       // longest row that one group does (16 / 32 / 64 / 128: 713 / 622 / 606 / 642 us on the graph above)
 constexpr int kAtOnce = 4;          // steps (a row of B per group) that are copied and added up together
@@ -273,6 +275,7 @@ __device__ __forceinline__ void copy_row(uint32_t dst, const void* src, uint32_t
 //   begin(row, whole, piece, at, end)   every group begins a row (row < 0: the group has none), or, `whole`, all groups the
 //                            same one; its entries are at places below `end`, and the one at place p is entry at + p (both
 //                            only where Work::kPlaces)
+//   ahead(row)               the group's next row of the window, or -1 (only where Work::kPlaces)
 //   step(val, x)             an entry of the row (one that the group does not have has the value 0): x is the lane's share of
 //                            its row of B, as Share::floats takes it
 //   steps_done(k, in)        after four steps: k is the place of the first of them in the window; in: they are the group's
@@ -338,7 +341,7 @@ struct RowWalk {
         for (int t = 0; t < T; ++t)
           if (at[t] >= 0) v[t] = __ldg(a.vals + at[t]);
       }
-      if (a.scale) {
+      if (a.scale) {   // (as copies beside the rows of B, multiplied when they are used: 633 -> 651 us in 8 bits, more instructions)
         float s[T];
 #pragma unroll
         for (int t = 0; t < T; ++t) s[t] = v[t] != 0.f ? __ldg(a.scale + c[t]) : 0.f;
@@ -517,6 +520,7 @@ struct RowWalk {
       for (int p = 0; p < held; p += R) {
         const Batch now = batch(p);
         if (!whole || !begun || Work::kPlaces) work.begin(now.row, whole, piece, now.at, now.end);
+        if constexpr (Work::kPlaces) work.ahead(!whole && p + R + g < held ? row + (sm.sorted[p + R + g] & 31) : -1);
 #pragma unroll 1
         for (int k = 0; k < now.steps; ++k) {
           take(now.place(k), now.has(k));

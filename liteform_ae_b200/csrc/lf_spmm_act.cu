@@ -2,8 +2,8 @@
 //
 // What it has to move: the entries (8 bytes each), C and the residual once; what bounds it are the rows of B, one for each
 // entry, out of the L2 and, as far as B is larger than that, out of memory, and the instructions that unpack and add them.
-// 2^20 power-law rows with 13.2 M entries: 128 bfloat16 features 0.62 ms (3.4 GB of rows of B, 5.5 TB/s), the same in 8 bits
-// 0.69 ms; the entries, one read of B and C and the residual would take 0.14 and 0.12 ms.
+// 2^20 power-law rows with 13.2 M entries: 128 bfloat16 features 0.56 ms (3.4 GB of rows of B, 6.0 TB/s), the same in 8 bits
+// 0.63 ms; the entries, one read of B and C and the residual would take 0.14 and 0.12 ms.
 //
 // Two launches.  In the first a warp takes a range of entries and does the rows in it (lf_layer_rows.cuh); a group of
 // lanes that has summed up its row runs the epilogue on its registers, the residual having been fetched along with the rows
@@ -199,26 +199,26 @@ struct ActWork {
 };
 
 template <int DT, int G, int CH, bool IND, bool VIO>
-__global__ void __launch_bounds__(kWalkThreads, 640 / kWalkThreads)
+__global__ void __launch_bounds__(kWalkThreads, kWalkBlocks)
 spmm_csr_act_kernel(const __grid_constant__ ActArgs a) {
   using S = Share<DT, G, CH>;
   extern __shared__ __align__(16) unsigned char act_smem[];
-  WalkSmem* walks = reinterpret_cast<WalkSmem*>(act_smem);
-  float* bias = reinterpret_cast<float*>(walks + kWalkThreads / 32);
+  WalkSmem& walk = *reinterpret_cast<WalkSmem*>(act_smem);
+  float* bias = reinterpret_cast<float*>(act_smem + sizeof(WalkSmem));
   let_dependents_launch();
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int lane = threadIdx.x;
   const int f0 = blockIdx.y * S::kFeatures, nf = min(a.N - f0, S::kFeatures);
-  for (int f = threadIdx.x; f < S::kSpan; f += kWalkThreads) bias[f] = a.bias && f < nf ? get_any(a.bias, f0 + f, a.bias_dtype) : 0.f;
-  __syncthreads();
+  for (int f = lane; f < S::kSpan; f += 32) bias[f] = a.bias && f < nf ? get_any(a.bias, f0 + f, a.bias_dtype) : 0.f;
+  __syncwarp();
   RowStarts ptr;
   ptr.init(a.indptr, a.rows, a.nnz);
-  const int64_t q = (int64_t)blockIdx.x * (kWalkThreads / 32) + w;
+  const int64_t q = blockIdx.x;
   if ((q << a.lg) >= ptr.total) return;
   const WalkArgs wa{a.indices + ptr.base, a.data && !a.order ? a.data + ptr.base : a.data, a.order ? a.order + ptr.base : nullptr, a.b_scale,
                     reinterpret_cast<const char*>(a.B) + (int64_t)f0 * dtype_bytes(DT), a.pitch_b, nf};
   const int first = S::feature(0, lane % G);
   ActWork<DT, G, CH, VIO> work{a, bias + first, 2 * q, f0, nf, f0 + first, nf - first, lane % G, !S::kShifted && a.vec && a.N % ActWork<DT, G, CH, VIO>::kBlock == 0};
-  RowWalk<DT, G, CH, IND, ActWork<DT, G, CH, VIO>>(wa, ptr, walks[w], work).range(q, a.lg, a.slack);
+  RowWalk<DT, G, CH, IND, ActWork<DT, G, CH, VIO>>(wa, ptr, walk, work).range(q, a.lg, a.slack);
 }
 
 // Rows without entries, and rows that several ranges share: their pieces in order.  Most of its time goes into looking
@@ -321,10 +321,10 @@ template <int DT, int G, int CH, bool IND, bool VIO>
 cudaError_t launch_walk_as(const ActArgs& a, cudaStream_t st) {
   using S = Share<DT, G, CH>;
   constexpr auto kernel = spmm_csr_act_kernel<DT, G, CH, IND, VIO>;
-  constexpr int smem = kWalkThreads / 32 * (int)sizeof(WalkSmem) + S::kSpan * 4;
+  constexpr int smem = (int)sizeof(WalkSmem) + S::kSpan * 4;
   const cudaError_t e = allow_smem<kernel>(smem);
   if (e != cudaSuccess) return e;
-  const dim3 grid((unsigned)ceil_div64(ceil_div64(a.nnz, (int64_t)1 << a.lg), kWalkThreads / 32), (unsigned)((a.N + S::kFeatures - 1) / S::kFeatures));
+  const dim3 grid((unsigned)ceil_div64(a.nnz, (int64_t)1 << a.lg), (unsigned)((a.N + S::kFeatures - 1) / S::kFeatures));
   kernel<<<grid, kWalkThreads, smem, st>>>(a);
   return cudaGetLastError();
 }
@@ -378,6 +378,8 @@ int lf_spmm_csr_act(const int64_t* indptr, const int32_t* indices, const float* 
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(LF_ERR_WORKSPACE_TOO_SMALL, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
   LF_REQUIRE((uintptr_t)workspace % 16 == 0, "the workspace must start on a 16-byte boundary");
+  LF_REQUIRE(nnz == 0 || (B != C && B != ep.preact), "B is read by all rows: C and preact must lie elsewhere");
+  LF_REQUIRE(C != ep.preact, "C and preact must not be the same");
   const int lg = range_log(nnz);
   LF_REQUIRE((nnz >> lg) < (1ll << 31) - 1, "too many entries");
   const bool vec = N % 8 == 0 && on_grid16(C, ldc, c_dtype) && (!ep.residual || on_grid16(ep.residual, ep.ld_residual, ep.residual_dtype)) &&

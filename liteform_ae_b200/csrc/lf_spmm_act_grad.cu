@@ -88,8 +88,9 @@ struct ValueGradArgs {
 // The group keeps its row of dZ in registers (computed there, not rounded) and multiplies the rows of B that come through the
 // ring with it; four dot products at a time are summed up over the lanes, each lane ending with one of them.  A row wider
 // than a walk takes several launches, which add to what the ones before wrote.  As in the product, the rows of B and the
-// instructions on them bound it (2^18 power-law rows, 3.1 M entries, 256 bfloat16 features, gelu: 455 us).
-template <int DT, int G, int CH>
+// instructions on them bound it (2^18 power-law rows, 3.1 M entries, 256 bfloat16 features, gelu: 300 us).
+// VIO: rows of dy and z have B's type and are known to be on the grid.
+template <int DT, int G, int CH, bool VIO>
 struct GradWork {
   using S = Share<DT, G, CH>;
   static constexpr bool kPlaces = true;
@@ -111,8 +112,33 @@ struct GradWork {
     const char* p = reinterpret_cast<const char*>(row_of_b(base, (uint32_t)row, pitch)) + f0 * bytes;
     for (int i = 0; i < nf * bytes; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + i));
   }
-  // the lane's features of a row, as floats; what lies behind its end is anything
-  __device__ __forceinline__ void load(const void* base, int row, uint32_t pitch, float* v) const {
+  // VIO: the group's next row is on its way while the steps of this one run (the case above took 455 us with one row of dy
+  // and one of z loaded after the other when they were needed, 341 with both at once then).
+  uint32_t wd[S::kFloats], wz[S::kFloats];
+  int held = -1;
+  __device__ __forceinline__ void fetch(int row) {
+    const int64_t at = f * dtype_bytes(DT);
+    load_blocks<S::kPieces, S::VEC>(reinterpret_cast<const char*>(row_of_b(a.dy, (uint32_t)row, a.pitch_dy)) + at, DT, kApart, left, wd);
+    if (a.z) load_blocks<S::kPieces, S::VEC>(reinterpret_cast<const char*>(row_of_b(a.z, (uint32_t)row, a.pitch_z)) + at, DT, kApart, left, wz);
+    held = row;
+  }
+  __device__ __forceinline__ void ahead(int row) {
+    if constexpr (VIO) {
+      if (row >= 0) fetch(row);
+    }
+  }
+  // the lane's features of rows of dy and z, as floats; what lies behind the rows' end is anything
+  __device__ __forceinline__ void load(int row, float* d, float* z) {
+    if constexpr (VIO) {
+      if (held != row) fetch(row);
+      use_blocks<S::kPieces, S::VEC>(wd, DT, d, [](float, float y) { return y; });
+      if (a.z) use_blocks<S::kPieces, S::VEC>(wz, DT, z, [](float, float y) { return y; });
+    } else {
+      load_any(a.dy, row, a.pitch_dy, d);
+      if (a.z) load_any(a.z, row, a.pitch_z, z);
+    }
+  }
+  __device__ __forceinline__ void load_any(const void* base, int row, uint32_t pitch, float* v) const {
     const char* p = reinterpret_cast<const char*>(row_of_b(base, (uint32_t)row, pitch)) + f * dtype_bytes(a.dy_dtype);
     if (vec) {
       __align__(16) uint32_t w[S::kFloats];
@@ -143,10 +169,9 @@ struct GradWork {
     used = 0;
     float d[S::kFloats];
     if (row >= 0) {
-      load(a.dy, row, a.pitch_dy, d);
+      float z[S::kFloats];
+      load(row, d, z);
       if (a.z) {
-        float z[S::kFloats];
-        load(a.z, row, a.pitch_z, z);
         slopes<S::kFloats>(z, a.act);
 #pragma unroll
         for (int i = 0; i < S::kFloats; ++i) d[i] *= z[i];
@@ -166,7 +191,7 @@ struct GradWork {
     S::floats(x, gl, y);
     // What lies behind the row's end may be anything, and a 0 in dz does not make up for it: a last piece that is not full is
     // cleared here, and pieces that no lane copies hold the zeros the kernel began with.
-    if (ragged) {
+    if (!VIO && ragged) {
 #pragma unroll
       for (int i = 0; i < S::kPairs; ++i) {
         const int k = 2 * i / kVec * kApart + 2 * i % kVec, k1 = (2 * i + 1) / kVec * kApart + (2 * i + 1) % kVec;
@@ -202,37 +227,46 @@ struct GradWork {
   __device__ __forceinline__ void end(int, bool, int) const {}
 };
 
-template <int DT, int G, int CH>
-__global__ void __launch_bounds__(kWalkThreads, 512 / kWalkThreads)   // dy, z and dz of a row at a time
+template <int DT, int G, int CH, bool VIO>
+__global__ void __launch_bounds__(kWalkThreads, kWalkBlocks)
 value_grad_kernel(const __grid_constant__ ValueGradArgs a) {
   using S = Share<DT, G, CH>;
   extern __shared__ __align__(16) unsigned char grad_smem[];
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, first = S::feature(0, lane % G);
+  const int lane = threadIdx.x, first = S::feature(0, lane % G);
   const int nf = min(a.N - a.f0, S::kFeatures);
   RowStarts ptr;
   ptr.init(a.indptr, a.rows, a.nnz);
-  const int64_t q = (int64_t)blockIdx.x * (kWalkThreads / 32) + w;
+  const int64_t q = blockIdx.x;
   if ((q << a.lg) >= ptr.total) return;
-  uint4* ring = reinterpret_cast<uint4*>(reinterpret_cast<WalkSmem*>(grad_smem)[w].ring);
+  WalkSmem& walk = *reinterpret_cast<WalkSmem*>(grad_smem);
+  uint4* ring = reinterpret_cast<uint4*>(walk.ring);
   for (int i = lane; i < kRingBytes / 16 + 1; i += 32) ring[i] = make_uint4(0u, 0u, 0u, 0u);
   __syncwarp();
   const WalkArgs wa{a.indices + ptr.base, nullptr, nullptr, nullptr, reinterpret_cast<const char*>(a.B) + (int64_t)a.f0 * dtype_bytes(DT), a.pitch_b, nf};
-  GradWork<DT, G, CH> work{a, a.f0, nf, a.f0 + first, nf - first, lane % G, S::kShifted || a.N % S::VEC != 0, !S::kShifted && a.vec && a.N % S::VEC == 0};
-  RowWalk<DT, G, CH, false, GradWork<DT, G, CH>>(wa, ptr, reinterpret_cast<WalkSmem*>(grad_smem)[w], work).range(q, a.lg, a.slack);
+  GradWork<DT, G, CH, VIO> work{a, a.f0, nf, a.f0 + first, nf - first, lane % G, S::kShifted || a.N % S::VEC != 0, !S::kShifted && a.vec && a.N % S::VEC == 0};
+  RowWalk<DT, G, CH, false, GradWork<DT, G, CH, VIO>>(wa, ptr, walk, work).range(q, a.lg, a.slack);
+}
+
+template <int DT, int G, int CH, bool VIO>
+cudaError_t launch_value_grad_as(ValueGradArgs a, cudaStream_t st) {
+  constexpr auto kernel = value_grad_kernel<DT, G, CH, VIO>;
+  constexpr int smem = (int)sizeof(WalkSmem);
+  cudaError_t e = allow_smem<kernel>(smem);
+  const unsigned grid = (unsigned)ceil_div64(a.nnz, (int64_t)1 << a.lg);
+  for (a.f0 = 0; a.f0 < a.N && e == cudaSuccess; a.f0 += Share<DT, G, CH>::kFeatures) {
+    kernel<<<grid, kWalkThreads, smem, st>>>(a);
+    e = cudaGetLastError();
+  }
+  return e;
 }
 
 template <int DT>
-cudaError_t launch_value_grad(ValueGradArgs a, cudaStream_t st) {
+cudaError_t launch_value_grad(const ValueGradArgs& a, cudaStream_t st) {
   return with_row_shape<DT>((uintptr_t)a.B % 16 == 0 && a.pitch_b % 16 == 0, a.N, [&](auto G, auto CH) {
-    constexpr auto kernel = value_grad_kernel<DT, G.value, CH.value>;
-    constexpr int smem = kWalkThreads / 32 * (int)sizeof(WalkSmem);
-    cudaError_t e = allow_smem<kernel>(smem);
-    const unsigned grid = (unsigned)ceil_div64(ceil_div64(a.nnz, (int64_t)1 << a.lg), kWalkThreads / 32);
-    for (a.f0 = 0; a.f0 < a.N && e == cudaSuccess; a.f0 += Share<DT, G.value, CH.value>::kFeatures) {
-      kernel<<<grid, kWalkThreads, smem, st>>>(a);
-      e = cudaGetLastError();
+    if constexpr (CH.value > 0) {
+      if (a.vec && a.dy_dtype == DT && a.N % Share<DT, G.value, CH.value>::VEC == 0) return launch_value_grad_as<DT, G.value, CH.value, true>(a, st);
     }
-    return e;
+    return launch_value_grad_as<DT, G.value, CH.value, false>(a, st);
   });
 }
 

@@ -79,6 +79,12 @@ def test_product_workspace_off_the_grid():
     assert product(ws=P + 4) == BAD
 
 
+@pytest.mark.parametrize("kw", [dict(B=P, C=P), dict(B=P, C=2 * P, ep=dict(preact=P, ld_preact=8)),
+                                dict(B=P, C=2 * P, ep=dict(preact=2 * P, ld_preact=8))])
+def test_product_outputs_lie_apart(kw):
+    assert product(**kw) == BAD and b"must" in _cabi.load().lf_last_error()
+
+
 def test_product_of_no_rows_does_nothing():
     assert product(r1=0, indptr=0, C=0) == 0
 
