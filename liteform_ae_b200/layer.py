@@ -236,6 +236,9 @@ class CsrTranspose:
         M, K = int(shape[0]), int(shape[1])
         indptr, indices = np.asarray(indptr, dtype=np.int64), np.asarray(indices)
         _need(len(indices) < 2 ** 31 and M < 2 ** 31, "at most 2^31 - 1 entries and rows")
+        _need(len(indptr) == M + 1 and indptr[0] == 0 and indptr[-1] == len(indices) and bool((np.diff(indptr) >= 0).all()),
+              "indptr must ascend from 0 to the number of entries")
+        _need(len(indices) == 0 or (indices.min() >= 0 and indices.max() < K), "columns must lie in the matrix")
         order = np.argsort(indices, kind="stable")
         rows = np.repeat(np.arange(M, dtype=np.int32), np.diff(indptr))[order]
         ptr = np.zeros(K + 1, dtype=np.int64)
@@ -254,14 +257,22 @@ def _csr_arrays(a, values, dev):
     transposed = isinstance(a, CsrTranspose)
     _need(transposed or values is None, "values go with a CsrTranspose; a DeviceCsr has its own")
     data = values if transposed else a.data
-    _need(a.indptr.get_device() == dev and a.indptr.is_contiguous() and a.indptr.numel() == a.shape[0] + 1,
-          "indptr must be a dense vector of one more than the rows, beside B")
-    _need(a.indices.get_device() == dev and a.indices.is_contiguous(), "indices must be a dense vector beside B")
+    torch = _torch()
+    indptr, indices = a.indptr, a.indices
+    _need(indptr.get_device() == dev and indptr.is_contiguous() and indptr.numel() == a.shape[0] + 1 and indptr.dtype == torch.int64,
+          "indptr must be a dense int64 vector of one more than the rows, beside B")
+    _need(indices.get_device() == dev and indices.is_contiguous() and indices.dtype == torch.int32,
+          "indices must be a dense int32 vector beside B")
     if data is None:
         return 0, 0
-    _need(data.numel() == a.nnz and data.is_contiguous() and data.get_device() == dev and data.dtype == _torch().float32,
+    _need(data.numel() == a.nnz and data.is_contiguous() and data.get_device() == dev and data.dtype == torch.float32,
           "the values must be a dense float32 vector, one per entry, beside B")
-    return data.data_ptr(), a.order.data_ptr() if transposed else 0
+    if not transposed:
+        return data.data_ptr(), 0
+    order = a.order
+    _need(order.get_device() == dev and order.is_contiguous() and order.dtype == torch.int32 and order.numel() == a.nnz,
+          "order must be a dense int32 vector, one per entry, beside B")
+    return data.data_ptr(), order.data_ptr()
 
 
 def spmm_csr_act(a, B, scale=None, bias=None, activation: Optional[str] = None, residual=None, out_dtype=None, out=None,
@@ -344,7 +355,8 @@ def act_backward(dy, preact=None, activation: Optional[str] = None, dz=None, nee
 
 def spmm_csr_grad_values(a: DeviceCsr, B, dy, preact=None, activation: Optional[str] = None, out=None):
     """``lf_spmm_csr_grad_values``: the gradient of A's values, ``dvalues[e] = <dz[row of e], B[column of e]>`` with
-    ``dz = dy * activation'(preact)`` not rounded in between; float32, one per entry."""
+    ``dz = dy * activation'(preact)`` not rounded in between; float32, one per entry.  For a ``DeviceCsr`` of a slice of
+    ``indptr`` the entries count from the slice's first, and what is behind its last is left as it is."""
     torch = _torch()
     K, N, dev = _first(B, "B")
     M = a.shape[0]

@@ -153,3 +153,10 @@ def test_slopes_by_differences(name):
     d = 1e-5
     diff = (ref.act(z + d, name) - ref.act(z - d, name)) / (2 * d)
     assert float((diff - ref.slope(z, name)).abs().max()) < 1e-8
+
+
+@pytest.mark.parametrize("indptr, indices, shape", [([0, 1, 3], [0, 1], (2, 4)), ([1, 1, 2], [0, 1], (2, 4)), ([0, 2], [0, 1], (2, 4)),
+                                                    ([0, 3, 2], [0, 1], (2, 4)), ([0, 1, 2], [0, 4], (2, 4)), ([0, 1, 2], [-1, 0], (2, 4))])
+def test_transposed_pattern_refusals(indptr, indices, shape):
+    with pytest.raises(ValueError):
+        layer.CsrTranspose.from_host(np.array(indptr), np.array(indices), shape, "cpu")

@@ -724,3 +724,33 @@ def test_infer(cuda_device):
         assert torch.equal(got, y)
     with pytest.raises(ValueError):
         pipeline.infer(m, x, [])
+
+
+def test_pattern_types_are_checked(cuda_device):
+    p = pattern(20, 30, 1)
+    A = csr_on(cuda_device, p, (20, 30))
+    T = layer.CsrTranspose.of(A)
+    B, Bt = torch.randn(30, 16, device=cuda_device), torch.randn(20, 16, device=cuda_device)
+    with_order = lambda order: layer.CsrTranspose(T.indptr, T.indices, order, T.shape)
+    for f in (lambda: layer.spmm_csr_act(hyb.DeviceCsr(A.indptr.int(), A.indices, A.data, A.shape), B),
+              lambda: layer.spmm_csr_act(hyb.DeviceCsr(A.indptr, A.indices.long(), A.data, A.shape), B),
+              lambda: layer.spmm_csr_grad_values(hyb.DeviceCsr(A.indptr, A.indices.long(), A.data, A.shape), B, Bt),
+              lambda: layer.spmm_csr_act(with_order(T.order.long()), Bt, values=A.data),
+              lambda: layer.spmm_csr_act(with_order(T.order[:-1]), Bt, values=A.data),
+              lambda: layer.spmm_csr_act(with_order(T.order.cpu()), Bt, values=A.data)):
+        with pytest.raises(ValueError):
+            f()
+
+
+def test_value_gradient_of_a_slice(cuda_device):
+    p = pattern(40, 30, 2)
+    A = csr_on(cuda_device, p, (40, 30))
+    B, dy = torch.randn(30, 16, device=cuda_device), torch.randn(40, 16, device=cuda_device)
+    full = layer.spmm_csr_grad_values(A, B, dy)
+    r0, r1 = 11, 29
+    e0, e1 = int(A.indptr[r0]), int(A.indptr[r1])
+    out = torch.full((A.nnz,), 7.0, device=cuda_device)
+    layer.spmm_csr_grad_values(hyb.DeviceCsr(A.indptr[r0:r1 + 1], A.indices, A.data, (r1 - r0, 30)), B, dy[r0:r1], out=out)
+    # the same products, perhaps added up in another order: 16 terms, each sum rounded
+    off = 16 * 2.0 ** -24 * (dy.abs().amax() * B.abs().amax()) * 16
+    assert (out[:e1 - e0] - full[e0:e1]).abs().max() <= off and (out[e1 - e0:] == 7.0).all()
