@@ -3,7 +3,7 @@
 // What it has to move: the entries (8 bytes each), C and the residual once; what bounds it are the rows of B, one for each
 // entry, out of the L2 and, as far as B is larger than that, out of memory, and the instructions that unpack and add them.
 // 2^20 power-law rows with 13.2 M entries: 128 bfloat16 features 0.56 ms (3.4 GB of rows of B, 6.0 TB/s), the same in 8 bits
-// 0.63 ms; the entries, one read of B and C and the residual would take 0.14 and 0.12 ms.
+// 0.60 ms; the entries, one read of B and C and the residual would take 0.14 and 0.12 ms.
 //
 // Two launches.  In the first a warp takes a range of entries and does the rows in it (lf_layer_rows.cuh); a group of
 // lanes that has summed up its row runs the epilogue on its registers, the residual having been fetched along with the rows
@@ -156,11 +156,18 @@ struct ActWork {
   }
   static constexpr bool kPlaces = false;
   __device__ __forceinline__ bool vec() const { return VIO || vec_; }
+  // The residual is on its way while the row is summed up, where its words take no more registers than the sums' rows of B; 16
+  // bits of either kind are loaded alike.  (Any residual so, 16 words held for 8
+  // used: the 8-bit case above 630 us for 596.)
+  __device__ __forceinline__ const char* residual_of(int row) const { return row_at(a.residual, row, a.pitch_res) + f * dtype_bytes(a.res_dtype); }
+  __device__ __forceinline__ bool early() const { return !S::kShifted && a.residual && vec() && (DT == LF_DTYPE_F32 || a.res_dtype != LF_DTYPE_F32); }
   __device__ __forceinline__ void begin(int row, bool whole, int piece, int64_t, int) {
 #pragma unroll
     for (int i = 0; i < S::kPairs; ++i) sum[i] = 0;
-    if (a.residual && row >= 0 && !(whole && piece >= 0))   // on its way while the row is summed up
-      Io::load(row_at(a.residual, row, a.pitch_res) + f * dtype_bytes(a.res_dtype), a.res_dtype, vec(), kApart, left, res);
+    if constexpr (!S::kShifted) {
+      if (early() && row >= 0 && !(whole && piece >= 0))
+        load_blocks<kBlocks, kBlock>(residual_of(row), DT == LF_DTYPE_F32 ? a.res_dtype : LF_DTYPE_BF16, kApart, left, res);
+    }
   }
   __device__ __forceinline__ void step(float v, const unsigned char* x) {
     uint64_t y[S::kPairs];
@@ -193,6 +200,7 @@ struct ActWork {
       for (int i = 0; i < S::kFloats; ++i)
         if (i / kBlock * kApart + i % kBlock < left) p[i / kBlock * kApart + i % kBlock] = z[i];
     } else {
+      if (a.residual && !early()) Io::load(residual_of(row), a.res_dtype, vec(), kApart, left, res);
       Io::finish(a, vec(), row, f, kApart, left, bias, res, z);
     }
   }
