@@ -131,8 +131,8 @@ __device__ __forceinline__ void finish8(const ActArgs& a, int row, int f, const 
 }
 
 // ---- the walk ---------------------------------------------------------------------------------------
-// VIO: rows of C, residual and preact are known to be on the grid.  Only the 8-bit form is compiled for that (2^20 uniform
-// rows of 64 features 790 -> 724 us, the shorter code); the 16-bit one is slower so (2^20 power-law rows 624 -> 687).
+// VIO: rows of C, residual and preact are known to be on the grid (2^20 power-law rows, 128 bfloat16 features 566 us without, 551
+// with; 2^20 uniform rows of 64 features in 8 bits 790 and 724).
 template <int DT, int G, int CH, bool VIO>
 struct ActWork {
   using S = Share<DT, G, CH>;
@@ -157,8 +157,8 @@ struct ActWork {
   static constexpr bool kPlaces = false;
   __device__ __forceinline__ bool vec() const { return VIO || vec_; }
   // The residual is on its way while the row is summed up, where its words take no more registers than the sums' rows of B; 16
-  // bits of either kind are loaded alike.  (Any residual so, 16 words held for 8
-  // used: the 8-bit case above 630 us for 596.)
+  // bits of either kind are loaded alike.  (Any residual so, 16 words held for 8 used:
+  // the 8-bit case above 630 us for 596.)
   __device__ __forceinline__ const char* residual_of(int row) const { return row_at(a.residual, row, a.pitch_res) + f * dtype_bytes(a.res_dtype); }
   __device__ __forceinline__ bool early() const { return !S::kShifted && a.residual && vec() && (DT == LF_DTYPE_F32 || a.res_dtype != LF_DTYPE_F32); }
   __device__ __forceinline__ void begin(int row, bool whole, int piece, int64_t, int) {
@@ -340,10 +340,17 @@ cudaError_t launch_walk_as(const ActArgs& a, cudaStream_t st) {
 template <int DT>
 cudaError_t launch_walk(const ActArgs& a, cudaStream_t st) {
   return with_row_shape<DT>((uintptr_t)a.B % 16 == 0 && a.pitch_b % 16 == 0, a.N, [&](auto G, auto CH) {
+    const bool plain = DT != LF_DTYPE_E4M3 && !a.b_scale && !a.order;
+    if constexpr (CH.value > 0) {
+      if (a.vec && a.N % ActWork<DT, G.value, CH.value, true>::kBlock == 0) {
+        if constexpr (DT != LF_DTYPE_E4M3) {
+          if (plain) return launch_walk_as<DT, G.value, CH.value, false, true>(a, st);
+        }
+        return launch_walk_as<DT, G.value, CH.value, true, true>(a, st);
+      }
+    }
     if constexpr (DT != LF_DTYPE_E4M3) {
-      if (!a.b_scale && !a.order) return launch_walk_as<DT, G.value, CH.value, false, false>(a, st);
-    } else if constexpr (CH.value > 0) {
-      if (a.vec && a.N % ActWork<DT, G.value, CH.value, true>::kBlock == 0) return launch_walk_as<DT, G.value, CH.value, true, true>(a, st);
+      if (plain) return launch_walk_as<DT, G.value, CH.value, false, false>(a, st);
     }
     return launch_walk_as<DT, G.value, CH.value, true, false>(a, st);
   });
