@@ -2,8 +2,8 @@
 //
 // What it has to move: the entries (8 bytes each), C and the residual once; what bounds it are the rows of B, one for each
 // entry, out of the L2 and, as far as B is larger than that, out of memory, and the instructions that unpack and add them.
-// 2^20 power-law rows with 13.2 M entries: 128 bfloat16 features 0.56 ms (3.4 GB of rows of B, 6.0 TB/s), the same in 8 bits
-// 0.60 ms; the entries, one read of B and C and the residual would take 0.14 and 0.12 ms.
+// 2^20 power-law rows with 13.2 M entries: 128 bfloat16 features 0.54 ms (3.4 GB of rows of B, 6.3 TB/s), the same in 8 bits
+// 0.58 ms; the entries, one read of B and C and the residual would take 0.14 and 0.12 ms.
 //
 // Two launches.  In the first a warp takes a range of entries and does the rows in it (lf_layer_rows.cuh); a group of
 // lanes that has summed up its row runs the epilogue on its registers, the residual having been fetched along with the rows
@@ -110,30 +110,35 @@ struct RowIo {
     }
   }
   // z = A * B for features f on, `bias` theirs, w their residual -> what the call returns
-  static __device__ __forceinline__ void finish(const ActArgs& a, bool vec, int row, int f, int apart, int left, const float* bias, const uint32_t* w, float* z) {
+  static __device__ __forceinline__ void finish(const ActArgs& a, int c_dtype, int res_dtype, bool vec, int row, int f, int apart, int left, const float* bias, const uint32_t* w, float* z) {
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b) {
 #pragma unroll
       for (int i = 0; i < n; ++i) z[b * n + i] += bias[b * apart + i];
     }
-    const int at = f * dtype_bytes(a.c_dtype);
-    if (a.preact) store(row_at(a.preact, row, a.pitch_pre) + at, a.c_dtype, vec, apart, left, z);
+    const int at = f * dtype_bytes(c_dtype);
+    if (a.preact) store(row_at(a.preact, row, a.pitch_pre) + at, c_dtype, vec, apart, left, z);
     activate_all<BLOCKS * n>(z, a.act);
-    if (a.residual) add(w, a.res_dtype, vec, z);
-    store(row_at(a.C, row, a.pitch_c) + at, a.c_dtype, vec, apart, left, z);
+    if (a.residual) add(w, res_dtype, vec, z);
+    store(row_at(a.C, row, a.pitch_c) + at, c_dtype, vec, apart, left, z);
   }
 };
 // eight features, the residual fetched here
 __device__ __forceinline__ void finish8(const ActArgs& a, int row, int f, const float* bias, float* z) {
   __align__(16) uint32_t w[8];
   if (a.residual) RowIo<1, 8>::load(row_at(a.residual, row, a.pitch_res) + f * dtype_bytes(a.res_dtype), a.res_dtype, a.vec, 8, a.N - f, w);
-  RowIo<1, 8>::finish(a, a.vec, row, f, 8, a.N - f, bias, w, z);
+  RowIo<1, 8>::finish(a, a.c_dtype, a.res_dtype, a.vec, row, f, 8, a.N - f, bias, w, z);
 }
 
 // ---- the walk ---------------------------------------------------------------------------------------
-// VIO: rows of C, residual and preact are known to be on the grid (2^20 power-law rows, 128 bfloat16 features 566 us without, 551
-// with; 2^20 uniform rows of 64 features in 8 bits 790 and 724).
-template <int DT, int G, int CH, bool VIO>
+// What is known of C, residual and preact when the kernel is compiled (2^20 power-law rows, 128 bfloat16 features 566 us with
+// kAnyRows, 551 with kOnGrid, 540 with kTyped; in 8 bits 595 and 579 with the latter two; 2^20 uniform rows of 64 features in 8
+// bits 790 with the first and 724 with the second).  Other types than kTyped's are compiled for the grid only from 8 bits, where
+// there is no type of its own for C.
+enum Rows { kAnyRows, kOnGrid, kTyped };   // on the grid: on 16-byte boundaries and of whole pieces; typed: of kOwn as well
+template <int DT> constexpr int kOwn = DT == LF_DTYPE_E4M3 ? LF_DTYPE_BF16 : DT;
+
+template <int DT, int G, int CH, Rows IO>
 struct ActWork {
   using S = Share<DT, G, CH>;
   // the lane's share of a row in memory
@@ -155,18 +160,20 @@ struct ActWork {
     for (int i = 0; i < nf * bytes; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + i));
   }
   static constexpr bool kPlaces = false;
-  __device__ __forceinline__ bool vec() const { return VIO || vec_; }
+  __device__ __forceinline__ bool vec() const { return IO != kAnyRows || vec_; }
+  __device__ __forceinline__ int c_dtype() const { return IO == kTyped ? kOwn<DT> : a.c_dtype; }
+  __device__ __forceinline__ int res_dtype() const { return IO == kTyped ? kOwn<DT> : a.res_dtype; }
   // The residual is on its way while the row is summed up, where its words take no more registers than the sums' rows of B; 16
   // bits of either kind are loaded alike.  (Any residual so, 16 words held for 8 used:
   // the 8-bit case above 630 us for 596.)
-  __device__ __forceinline__ const char* residual_of(int row) const { return row_at(a.residual, row, a.pitch_res) + f * dtype_bytes(a.res_dtype); }
-  __device__ __forceinline__ bool early() const { return !S::kShifted && a.residual && vec() && (DT == LF_DTYPE_F32 || a.res_dtype != LF_DTYPE_F32); }
+  __device__ __forceinline__ const char* residual_of(int row) const { return row_at(a.residual, row, a.pitch_res) + f * dtype_bytes(res_dtype()); }
+  __device__ __forceinline__ bool early() const { return !S::kShifted && a.residual && vec() && (DT == LF_DTYPE_F32 || res_dtype() != LF_DTYPE_F32); }
   __device__ __forceinline__ void begin(int row, bool whole, int piece, int64_t, int) {
 #pragma unroll
     for (int i = 0; i < S::kPairs; ++i) sum[i] = 0;
     if constexpr (!S::kShifted) {
       if (early() && row >= 0 && !(whole && piece >= 0))
-        load_blocks<kBlocks, kBlock>(residual_of(row), DT == LF_DTYPE_F32 ? a.res_dtype : LF_DTYPE_BF16, kApart, left, res);
+        load_blocks<kBlocks, kBlock>(residual_of(row), DT == LF_DTYPE_F32 ? res_dtype() : LF_DTYPE_BF16, kApart, left, res);
     }
   }
   __device__ __forceinline__ void step(float v, const unsigned char* x) {
@@ -200,13 +207,13 @@ struct ActWork {
       for (int i = 0; i < S::kFloats; ++i)
         if (i / kBlock * kApart + i % kBlock < left) p[i / kBlock * kApart + i % kBlock] = z[i];
     } else {
-      if (a.residual && !early()) Io::load(residual_of(row), a.res_dtype, vec(), kApart, left, res);
-      Io::finish(a, vec(), row, f, kApart, left, bias, res, z);
+      if (a.residual && !early()) Io::load(residual_of(row), res_dtype(), vec(), kApart, left, res);
+      Io::finish(a, c_dtype(), res_dtype(), vec(), row, f, kApart, left, bias, res, z);
     }
   }
 };
 
-template <int DT, int G, int CH, bool IND, bool VIO>
+template <int DT, int G, int CH, bool IND, Rows IO>
 __global__ void __launch_bounds__(kWalkThreads, kWalkBlocks)
 spmm_csr_act_kernel(const __grid_constant__ ActArgs a) {
   using S = Share<DT, G, CH>;
@@ -225,8 +232,8 @@ spmm_csr_act_kernel(const __grid_constant__ ActArgs a) {
   const WalkArgs wa{a.indices + ptr.base, a.data && !a.order ? a.data + ptr.base : a.data, a.order ? a.order + ptr.base : nullptr, a.b_scale,
                     reinterpret_cast<const char*>(a.B) + (int64_t)f0 * dtype_bytes(DT), a.pitch_b, nf};
   const int first = S::feature(0, lane % G);
-  ActWork<DT, G, CH, VIO> work{a, bias + first, 2 * q, f0, nf, f0 + first, nf - first, lane % G, !S::kShifted && a.vec && a.N % ActWork<DT, G, CH, VIO>::kBlock == 0};
-  RowWalk<DT, G, CH, IND, ActWork<DT, G, CH, VIO>>(wa, ptr, walk, work).range(q, a.lg, a.slack);
+  ActWork<DT, G, CH, IO> work{a, bias + first, 2 * q, f0, nf, f0 + first, nf - first, lane % G, !S::kShifted && a.vec && a.N % ActWork<DT, G, CH, IO>::kBlock == 0};
+  RowWalk<DT, G, CH, IND, ActWork<DT, G, CH, IO>>(wa, ptr, walk, work).range(q, a.lg, a.slack);
 }
 
 // Rows without entries, and rows that several ranges share: their pieces in order.  Most of its time goes into looking
@@ -325,10 +332,10 @@ finish_rows_kernel(const __grid_constant__ ActArgs a, int span) {   // span: row
   }
 }
 
-template <int DT, int G, int CH, bool IND, bool VIO>
+template <int DT, int G, int CH, bool IND, Rows IO>
 cudaError_t launch_walk_as(const ActArgs& a, cudaStream_t st) {
   using S = Share<DT, G, CH>;
-  constexpr auto kernel = spmm_csr_act_kernel<DT, G, CH, IND, VIO>;
+  constexpr auto kernel = spmm_csr_act_kernel<DT, G, CH, IND, IO>;
   constexpr int smem = (int)sizeof(WalkSmem) + S::kSpan * 4;
   const cudaError_t e = allow_smem<kernel>(smem);
   if (e != cudaSuccess) return e;
@@ -340,19 +347,19 @@ cudaError_t launch_walk_as(const ActArgs& a, cudaStream_t st) {
 template <int DT>
 cudaError_t launch_walk(const ActArgs& a, cudaStream_t st) {
   return with_row_shape<DT>((uintptr_t)a.B % 16 == 0 && a.pitch_b % 16 == 0, a.N, [&](auto G, auto CH) {
-    const bool plain = DT != LF_DTYPE_E4M3 && !a.b_scale && !a.order;
+    const auto launch = [&](auto io) {
+      if constexpr (DT != LF_DTYPE_E4M3) {
+        if (!a.b_scale && !a.order) return launch_walk_as<DT, G.value, CH.value, false, io.value>(a, st);
+      }
+      return launch_walk_as<DT, G.value, CH.value, true, io.value>(a, st);
+    };
     if constexpr (CH.value > 0) {
-      if (a.vec && a.N % ActWork<DT, G.value, CH.value, true>::kBlock == 0) {
-        if constexpr (DT != LF_DTYPE_E4M3) {
-          if (plain) return launch_walk_as<DT, G.value, CH.value, false, true>(a, st);
-        }
-        return launch_walk_as<DT, G.value, CH.value, true, true>(a, st);
+      if (a.vec && a.N % ActWork<DT, G.value, CH.value, kTyped>::kBlock == 0) {
+        if (a.c_dtype == kOwn<DT> && (!a.residual || a.res_dtype == kOwn<DT>)) return launch(std::integral_constant<Rows, kTyped>());
+        if constexpr (DT == LF_DTYPE_E4M3) return launch(std::integral_constant<Rows, kOnGrid>());
       }
     }
-    if constexpr (DT != LF_DTYPE_E4M3) {
-      if (plain) return launch_walk_as<DT, G.value, CH.value, false, false>(a, st);
-    }
-    return launch_walk_as<DT, G.value, CH.value, true, false>(a, st);
+    return launch(std::integral_constant<Rows, kAnyRows>());
   });
 }
 
