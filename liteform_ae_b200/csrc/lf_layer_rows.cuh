@@ -21,10 +21,11 @@ namespace lf {
 
 // Entries of a warp's range: the most that still gives each of the chip's 148 SMs the 20 warps that it could hold, three times
 // over where there are enough, from 64 to 2048 (2^20 uniform rows, 33.5 M entries: 735 us with 1024 each, 707 with 2048; the
-// power-law rows above 620 with 512, 615 with 1024).
-inline int range_log(int64_t nnz) {
+// power-law rows above 620 with 512, 615 with 1024).  From 16 where most rows have no entry, since there each may take a search
+// for its row (332 469 rows with 40 entries: 196 us for 64, 85 for 16; 3497 rows with 56 000, some of them long: 27 and 34).
+inline int range_log(int64_t nnz, int64_t rows) {
   int lg = 11;
-  while (lg > 6 && (nnz >> lg) < 148 * 20 * (lg > 8 ? 3 : 1)) --lg;
+  while (lg > (rows > nnz ? 4 : 6) && (nnz >> lg) < 148 * 20 * (lg > 8 ? 3 : 1)) --lg;
   return lg;
 }
 // A row that starts in a range and ends at most so far behind its nominal end belongs to it whole; only longer ones are

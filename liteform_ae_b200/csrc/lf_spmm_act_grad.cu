@@ -331,7 +331,7 @@ int lf_spmm_csr_grad_values(const int64_t* indptr, const int32_t* indices, int64
   if (row_begin == row_end || nnz == 0) return LF_OK;
   LF_REQUIRE(indptr && indices && dy && B && dvalues, "null pointer argument");
   LF_REQUIRE(activation == LF_ACT_NONE || (preact && ld_preact >= N && ld_preact < (1ll << 30)), "preact missing");
-  const int lg = range_log(nnz);
+  const int lg = range_log(nnz, row_end - row_begin);
   LF_REQUIRE((nnz >> lg) < (1ll << 31) - 1, "too many entries");
   const uint32_t bytes = (uint32_t)dtype_bytes(dy_dtype);
   const ValueGradArgs a{indptr + row_begin, indices, nnz, dy, activation == LF_ACT_NONE ? nullptr : preact, B, dvalues,

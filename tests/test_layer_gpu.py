@@ -754,3 +754,25 @@ def test_value_gradient_of_a_slice(cuda_device):
     # the same products, perhaps added up in another order: 16 terms, each sum rounded
     off = 16 * 2.0 ** -24 * (dy.abs().amax() * B.abs().amax()) * 16
     assert (out[:e1 - e0] - full[e0:e1]).abs().max() <= off and (out[e1 - e0:] == 7.0).all()
+
+
+@pytest.mark.parametrize("N", [16, 40, 47])
+@pytest.mark.parametrize("dtype,out", [(F32, F32), (BF16, BF16), (E4M3, BF16), (E4M3, F32)])
+def test_mostly_empty_rows(cuda_device, N, dtype, out):
+    M, K = 20000, 300
+    g = gen(N)
+    p = pattern(M, K, N, 0.003, 200, empty=0.0)
+    assert 200 < len(p[1]) < 400
+    A = csr_on(cuda_device, p, (M, K))
+    B, scale, Bv = features(K, N, dtype, g, cuda_device)
+    R, Rv = rows_of((M, N), out, g, cuda_device)
+    _, y, _, yoff = ref.product(ref.dense(*p, (M, K)), Bv, None, "silu", Rv, out)
+    ref.close(layer.spmm_csr_act(A, B, scale=scale, activation="silu", residual=R, out_dtype=out), y, yoff, "y")
+    if dtype == E4M3:
+        return
+    dy, dyv = rows_of((M, N), out, g, cuda_device)
+    rows = torch.repeat_interleave(torch.arange(M), torch.diff(p[0]))
+    terms = dyv[rows] * Bv[p[1].long()]
+    # N products, each rounded, and their sums: N units of the magnitudes' sum cover both
+    off = (N + 1) * 2.0 ** -24 * terms.abs().sum(1)
+    ref.close(layer.spmm_csr_grad_values(A, B, dy), terms.sum(1), off, "dvalues")
