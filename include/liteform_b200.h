@@ -479,9 +479,11 @@ int lf_spmm_csr_grad_values(const int64_t* indptr /*[dev]*/, const int32_t* indi
 
 /* h = x + residual rounded to `dtype` (the sum is kept in `sum`, which may be x or residual itself; without
  * a residual h = x and sum is not used), rstd = (mean(h^2) + eps)^(-1/2), y = h * rstd * weight in y_dtype.  For
- * e4m3 scale[r] = max|y[r,:]| / 448 and y holds y / scale; a row whose largest magnitude is below 448 * 2^-126
+ * e4m3 scale[r] = max|y[r,:]| / 448 and y holds y / scale = 448 h weight / max|h weight|, rounded from that quotient
+ * (rightly to the last one where x and weight are bfloat16); a row whose largest magnitude is below 448 * 2^-126
  * is stored as zeros with scale 0, a row with a NaN gets the scale NaN.  rstd: one float per row for the
- * backward pass, or NULL. */
+ * backward pass, or NULL.  The squares are added up in 32 bits: rows of numbers beyond about 10^19 / sqrt(N) come out
+ * as 0 or, in 8 bits, NaN. */
 int lf_rms_norm(const void* x /*[dev]*/, int32_t dtype, int64_t ld_x, const void* residual /*[dev] or NULL*/,
                 int64_t ld_residual, void* sum /*[dev] out*/, int64_t ld_sum, const void* weight /*[dev] N*/,
                 int32_t weight_dtype, float eps, void* y /*[dev] out*/, int32_t y_dtype, int64_t ld_y,

@@ -40,14 +40,34 @@ __device__ __forceinline__ float block_max(float v, float* smem) {
   return v;
 }
 
-// what a row is multiplied with before it is rounded to e4m3; rows whose largest magnitude is below
-// 448 * 2^-126 count as zero
-__device__ __forceinline__ float e4m3_scale(float amax, float* inverse) {
-  const float scale = amax * (1.f / 448.f);
-  const bool zero = scale < 1.17549435e-38f;
-  *inverse = zero ? 0.f : __fdividef(1.f, scale);   // within an ulp, and scale is far below 2^126
-  return zero ? 0.f : scale;
-}
+// Rows of e4m3.  y / scale = 448 h w / max|h w| has no rstd in it, so it is made from p = h (448 w) alone, which is exact for
+// bfloat16 rows and weights: halves between two stored values, frequent among numbers of few bits, go to the even one (from y =
+// h rstd w and a reciprocal of the scale 17 000 of 134 million went to the other).  Rows whose largest |y| is below 448 * 2^-126
+// count as zero.
+struct E4m3Row {
+  float scale;     // what the stored values are multiples of
+  float top;       // max|h w|
+  float inverse;   // 1 / top, or 0 for a row of zeros
+  __device__ __forceinline__ E4m3Row(float most, float rstd) {   // most: the largest |p|
+    top = __fdiv_rn(most, 448.f);
+    scale = rstd * top * (1.f / 448.f);
+    const bool zero = scale < 1.17549435e-38f;   // a NaN is none
+    inverse = zero ? 0.f : __frcp_rn(top);
+    if (zero) scale = 0.f;
+  }
+  // A top so small that its reciprocal may overflow (only beside an eps far below 10^-30): p and top are taken 2^100-fold.
+  __device__ __forceinline__ bool tiny() const { return top < 0x1p-100f; }
+  __device__ __forceinline__ float lift() {
+    top *= 0x1p100f;
+    if (inverse != 0.f) inverse = __frcp_rn(top);
+    return 0x1p100f;
+  }
+  // p / top: a product with the reciprocal, and what is left of p added
+  __device__ __forceinline__ float quotient(float p) const {
+    const float t = p * inverse;
+    return fmaf(fmaf(-t, top, p), inverse, t);
+  }
+};
 
 // One block per row, element by element: any size, stride and alignment.
 template <int DT>
@@ -72,21 +92,20 @@ rms_norm_rows_kernel(NormArgs a) {
     const float rstd = rsqrtf(block_sum(ss, smem) / (float)a.N + a.eps);
     if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
     const auto* h = a.res ? sum : x;   // a thread reads what it wrote itself
-    float inverse = 1.f;
-    if (a.y_dtype == LF_DTYPE_E4M3) {
-      float amax = 0.f;
+    if (a.y_dtype != LF_DTYPE_E4M3) {
       for (int f = threadIdx.x; f < a.N; f += 256)
-        amax = max_nan(amax, fabsf(T::get(h[f]) * rstd * get_any(a.weight, f, a.weight_dtype)));
-      const float scale = e4m3_scale(block_max(amax, smem), &inverse);
-      if (threadIdx.x == 0) a.scale[row] = scale;
+        put_any(a.y, row * a.ld_y + f, a.y_dtype, T::get(h[f]) * rstd * get_any(a.weight, f, a.weight_dtype));
+      continue;
     }
-    for (int f = threadIdx.x; f < a.N; f += 256) {
-      const float y = T::get(h[f]) * rstd * get_any(a.weight, f, a.weight_dtype);
-      if (a.y_dtype == LF_DTYPE_E4M3)
-        reinterpret_cast<__nv_fp8_storage_t*>(a.y)[row * a.ld_y + f] = Type<LF_DTYPE_E4M3>::put(y * inverse);
-      else
-        put_any(a.y, row * a.ld_y + f, a.y_dtype, y);
-    }
+    float most = 0.f;
+    for (int f = threadIdx.x; f < a.N; f += 256)
+      most = max_nan(most, fabsf(T::get(h[f]) * (448.f * get_any(a.weight, f, a.weight_dtype))));
+    E4m3Row to(block_max(most, smem), rstd);
+    if (threadIdx.x == 0) a.scale[row] = to.scale;
+    const float lift = to.tiny() ? to.lift() : 1.f;
+    auto* y = reinterpret_cast<__nv_fp8_storage_t*>(a.y) + row * a.ld_y;
+    for (int f = threadIdx.x; f < a.N; f += 256)
+      y[f] = Type<LF_DTYPE_E4M3>::put(to.quotient(T::get(h[f]) * (448.f * get_any(a.weight, f, a.weight_dtype)) * lift));
   }
 }
 
@@ -149,7 +168,7 @@ rms_norm_kernel(NormArgs a) {
 #pragma unroll
   for (int c = 0; c < C; ++c) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) w[c][i] = c * L * VEC < left ? get_any(a.weight, (t + c * L) * VEC + i, a.weight_dtype) : 0.f;
+    for (int i = 0; i < VEC; ++i) w[c][i] = c * L * VEC < left ? (OUT == LF_DTYPE_E4M3 ? 448.f : 1.f) * get_any(a.weight, (t + c * L) * VEC + i, a.weight_dtype) : 0.f;
   }
   int64_t row = (int64_t)blockIdx.x * GROUPS + group;
   const int64_t step = (int64_t)gridDim.x * GROUPS;
@@ -193,28 +212,42 @@ rms_norm_kernel(NormArgs a) {
     if (AHEAD) fetch(row + step < a.rows);
     const float rstd = rsqrtf(row_reduce<L, false>(ss, smem) * inv_n + a.eps);
     if (a.rstd && t == 0 && ok) a.rstd[row] = rstd;
-    float amax = 0.f;
+    if constexpr (OUT == LF_DTYPE_E4M3) {
+      float most = 0.f;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        float mc = 0.f;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          y[c][i] *= w[c][i];
+          mc = max_nan(mc, fabsf(y[c][i]));
+        }
+        if (c * L * VEC < left) most = max_nan(most, mc);
+      }
+      E4m3Row to(row_reduce<L, true>(most, smem), rstd);
+      if (t == 0 && ok) a.scale[row] = to.scale;
+      if (to.tiny()) {
+        const float lift = to.lift();
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) y[c][i] *= lift;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) y[c][i] = to.quotient(y[c][i]);
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) y[c][i] *= rstd * w[c][i];
+      }
+    }
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      float mc = 0.f;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        y[c][i] *= rstd * w[c][i];
-        if (OUT == LF_DTYPE_E4M3) mc = max_nan(mc, fabsf(y[c][i]));
-      }
-      if (c * L * VEC < left) amax = max_nan(amax, mc);
-    }
-    float inverse = 1.f;
-    if (OUT == LF_DTYPE_E4M3) {
-      const float scale = e4m3_scale(row_reduce<L, true>(amax, smem), &inverse);
-      if (t == 0 && ok) a.scale[row] = scale;
-    }
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      if (OUT == LF_DTYPE_E4M3) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) y[c][i] *= inverse;
-      }
       Pack<OUT, VEC> o;
       o.put(y[c]);
       if (ok && c * L * VEC < left) o.keep(py + c * L * VEC);

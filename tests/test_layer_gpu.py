@@ -776,3 +776,35 @@ def test_mostly_empty_rows(cuda_device, N, dtype, out):
     # N products, each rounded, and their sums: N units of the magnitudes' sum cover both
     off = (N + 1) * 2.0 ** -24 * terms.abs().sum(1)
     ref.close(layer.spmm_csr_grad_values(A, B, dy), terms.sum(1), off, "dvalues")
+
+
+@pytest.mark.parametrize("M,N,pitch", [(8000, 128, 128), (3000, 47, 47), (700, 1000, 1000), (200, 300, 301), (60, 4096, 4096), (40, 9000, 9001)])
+@pytest.mark.parametrize("residual", [False, True])
+def test_eight_bit_rows_are_rounded_to_nearest(cuda_device, M, N, pitch, residual):
+    """Stored is 448 h w / max|h w| to the nearest value, halves to the even one.  For bfloat16 h and w both products are
+    exact in 64 bits; a quotient that is a half is one there too (it has five bits), and any other is at least 2^-22 of itself
+    away from one: its two integers have 16 and 19 bits.  So the 64-bit quotient, through float32, rounds as the true one."""
+    g = gen(N)
+    x, xv = rows_of((M, N), BF16, g, cuda_device, pitch)
+    r, rv = rows_of((M, N), BF16, g, cuda_device, pitch) if residual else (None, None)
+    w = (1 + 0.1 * torch.randn(N, generator=g)).to(BF16).to(cuda_device)
+    n = layer.rms_norm(x, w, residual=r, out_dtype=E4M3)
+    p = n.h.cpu().double() * w.cpu().double()
+    want = (448 * p / p.abs().amax(1, keepdim=True)).float().to(E4M3).float()
+    got = n.y.cpu().float()
+    assert int((got != want).sum()) == 0
+
+
+def test_eight_bit_rows_of_tiny_numbers(cuda_device):
+    """A reciprocal of max|h w| would overflow; y itself is an ordinary number, since eps is smaller still."""
+    x = torch.randn(5, 64, generator=gen(1)) * torch.tensor([[1e-19], [1e-30], [1e-36], [1e-38], [0.0]])
+    w = torch.full((64,), 1e-9)
+    n = layer.rms_norm(x.to(cuda_device), w.to(cuda_device), eps=1e-37, out_dtype=E4M3)
+    y = x.double() * (x.double().square().mean(1, keepdim=True) + 1e-37) ** -0.5 * w.double()
+    y = torch.where(y.abs().amax(1, keepdim=True) < 448 * 2.0 ** -126, torch.zeros_like(y), y)
+    s = n.scale.cpu().double()[:, None]
+    back = n.y.cpu().double() * s
+    # half a step of 2^-4, 2^-10 of the scale below the normal numbers; h w itself is a subnormal number in the later rows, known to
+    # 2^-150 * rstd (below 2^-88 here); eps in 32 bits and the square's sum: 2^-20
+    off = 2.0 ** -4 * y.abs() * 1.01 + 2.0 ** -10 * s + 2.0 ** -88 + 2.0 ** -20 * y.abs()
+    assert bool(((back - y).abs() <= off).all()) and bool((back[4] == 0).all())
