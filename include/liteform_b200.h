@@ -449,7 +449,8 @@ typedef struct lf_epilogue {
  * nnz: the exact number of entries of the rows, for the workspace's size too (it does not grow
  * steadily).  The workspace holds the sums of rows that several thread groups share; it may be used
  * again as soon as the call is over on the stream, not by two calls at a time.  C and preact must not
- * lie in B, nor in each other.  Fewer than 2^31 rows, every stride below 2^30, at most 2^22 features.
+ * share memory with B or with each other, nor with a residual that is not the same rows: equal addresses
+ * are refused, other overlaps are the caller's to avoid (the Python calls compare the ranges).  Fewer than 2^31 rows, every stride below 2^30, at most 2^22 features.
  * Rows of B off the 16-byte grid are read in the aligned 16-byte pieces that cover them, as in
  * lf_spmm_csr_f32. */
 size_t lf_spmm_csr_act_workspace_bytes(int64_t nnz, int32_t N, int32_t b_dtype);

@@ -399,7 +399,7 @@ int lf_spmm_csr_act(const int64_t* indptr, const int32_t* indices, const float* 
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(LF_ERR_WORKSPACE_TOO_SMALL, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
   LF_REQUIRE((uintptr_t)workspace % 16 == 0, "the workspace must start on a 16-byte boundary");
-  LF_REQUIRE(nnz == 0 || (B != C && B != ep.preact), "B is read by all rows: C and preact must lie elsewhere");
+  LF_REQUIRE(nnz == 0 || (B != C && B != ep.preact), "C and preact must not start where B does, nor lie in it at all: every row reads B");
   LF_REQUIRE(C != ep.preact, "C and preact must not be the same");
   const int lg = range_log(nnz, row_end - row_begin);
   LF_REQUIRE((nnz >> lg) < (1ll << 31) - 1, "too many entries");

@@ -15,7 +15,8 @@ The reference has no counterpart: its product ends with C = A * B (playground_pi
 All computation is done by ``liblf_b200.so`` on torch's current stream of the tensors' device; nothing is
 synchronised (except for a ``row_range``, see ``spmm_csr_act``).  The same call on the same inputs gives the same
 bits.  Matrices are dense in their last dimension and may have any row stride of at least their width; a row stride
-and address on 16-byte boundaries is faster.  ``ValueError`` for arguments that do not fit together.
+and address on 16-byte boundaries is faster.  Outputs may not share memory with each other or with inputs, but for the
+matrices that a call names as allowed.  ``ValueError`` for arguments that do not fit together.
 """
 from __future__ import annotations
 
@@ -87,6 +88,38 @@ def _first(t, name):
     return t.shape[0], t.shape[1], t.get_device()
 
 
+def _extent(t):
+    """``(address, bytes of a row, bytes from a row to the next, rows)``; dense tensors count as one row."""
+    e = t.element_size()
+    if t.dim() != 2 or t.shape[0] < 2 or t.stride(0) == t.shape[1]:
+        return t.data_ptr(), t.numel() * e, 0, 1 if t.numel() else 0
+    return t.data_ptr(), t.shape[1] * e, t.stride(0) * e, t.shape[0]
+
+
+def _share_memory(a, b) -> bool:
+    """Whether two matrices or vectors have bytes in common.  Rows at one distance may lie beside each other, as column slices of a
+    buffer do; at two distances, one reaching into the other counts as sharing."""
+    (p, wide_a, step_a, n_a), (q, wide_b, step_b, n_b) = _extent(a), _extent(b)
+    if not n_a or not n_b or p + (n_a - 1) * step_a + wide_a <= q or q + (n_b - 1) * step_b + wide_b <= p:
+        return False
+    step = step_a or step_b
+    if not step or (step_a and step_b and step_a != step_b):
+        return True
+    gap = (q - p) % step       # from a row of a to the next of b
+    return gap < wide_a or gap + wide_b > step
+
+
+def _outputs_apart(given, inputs, may_be=()):
+    """Refuses outputs that the caller gave in memory that the call reads or writes elsewhere: ``given`` and ``inputs`` are
+    ``(tensor, name)``, tensors may be None; ``may_be``: pairs of names that may be one and the same matrix."""
+    given = [(t, name) for t, name in given if t is not None]
+    for i, (t, name) in enumerate(given):
+        for other, of in given[i + 1:] + [o for o in inputs if o[0] is not None]:
+            if _share_memory(t, other) and not ((name, of) in may_be and t.data_ptr() == other.data_ptr() and t.dtype == other.dtype
+                                                and t.shape == other.shape and t.stride() == other.stride()):
+                raise ValueError(f"{name} lies in the memory of {of}")
+
+
 def _act_code(activation):
     code = ACTIVATIONS.get(activation)
     if code is None:
@@ -148,9 +181,13 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, out_dtype=None, out=No
              rstd=None) -> NormOutput:
     """``lf_rms_norm``: ``h = x + residual`` in x's type, ``y = h * rstd * weight`` with ``rstd = (mean(h^2) +
     eps)^(-1/2)``, row by row.  ``out_dtype`` (default: x's): float32, bfloat16, float16, or float8_e4m3fn with one
-    scale per row (``y * scale`` is the row).  ``out``, ``scale``, ``sum_out`` (may be ``x`` or ``residual``) and
-    ``rstd`` take the outputs in place of new tensors."""
+    scale per row (``y * scale`` is the row).  ``out``, ``scale``, ``sum_out`` and ``rstd`` take the outputs in place of new
+    tensors; ``out`` and ``sum_out`` may each be ``x`` or ``residual`` itself."""
     torch = _torch()
+    if out is not None or sum_out is not None or scale is not None or rstd is not None:
+        _outputs_apart(((out, "out"), (sum_out, "sum_out"), (scale, "scale"), (rstd, "rstd")),
+                       ((x, "x"), (residual, "residual"), (weight, "weight")),
+                       {("out", "x"), ("out", "residual"), ("sum_out", "x"), ("sum_out", "residual")})
     M, N, dev = _first(x, "x")
     code = _code(x.dtype)
     ld_x = _matrix(x, "x", M, N, dev)
@@ -193,6 +230,9 @@ def rms_norm_backward(dy, h, weight, rstd, dh=None, dx=None, dweight=None, works
     float32.  For 8-bit rows pass the gradient of the rows they stand for (the rounding's own is taken as 1).
     ``dx`` may be ``dy``, ``h`` or ``dh``."""
     torch = _torch()
+    if dx is not None or dweight is not None:
+        _outputs_apart(((dx, "dx"), (dweight, "dweight")), ((dy, "dy"), (h, "h"), (dh, "dh"), (weight, "weight"), (rstd, "rstd")),
+                       {("dx", "dy"), ("dx", "h"), ("dx", "dh"), ("dweight", "weight")})
     lib = _cabi.load()
     M, N, dev = _first(dy, "dy")
     code = _code(dy.dtype)
@@ -285,6 +325,9 @@ def spmm_csr_act(a, B, scale=None, bias=None, activation: Optional[str] = None, 
     waits for the stream; a ``DeviceCsr`` of a slice of ``indptr`` does not.  Entries are not checked against B's rows:
     ``DeviceCsr.validate`` does that, once per matrix."""
     torch = _torch()
+    if out is not None or preact is not None:
+        _outputs_apart(((out, "out"), (preact, "preact")), ((B, "B"), (residual, "residual"), (bias, "bias"), (scale, "scale")),
+                       {("out", "residual"), ("preact", "residual")})
     lib = _cabi.load()
     K, N, dev = _first(B, "B")
     _need(K == a.shape[1], "B must have one row per matrix column")
@@ -311,7 +354,6 @@ def spmm_csr_act(a, B, scale=None, bias=None, activation: Optional[str] = None, 
         b_ptr, b_type = _vector(bias, "bias", N, dev), _code(bias.dtype)
     if residual is not None:
         r_ptr, r_type, ld_res = residual.data_ptr(), _code(residual.dtype), _matrix(residual, "residual", r1 - r0, N, dev)
-        _need(r_ptr != c_ptr or (residual.dtype == out_dtype and ld_res == ldc), "a residual at out's address must be out")
     if preact is not None:
         _need(preact.dtype == out_dtype, "preact must have the result's type")
         z_ptr, ld_z = preact.data_ptr(), _matrix(preact, "preact", r1 - r0, N, dev)
@@ -328,8 +370,10 @@ def spmm_csr_act(a, B, scale=None, bias=None, activation: Optional[str] = None, 
 def act_backward(dy, preact=None, activation: Optional[str] = None, dz=None, need_dz: bool = True, need_dbias: bool = True,
                  dbias=None, workspace: Optional[Workspace] = None):
     """``lf_act_backward``: ``(dz, dbias)`` with ``dz = dy * activation'(preact)`` in dy's type and ``dbias`` the float32
-    sum of its rows before they are rounded; what is not needed is None."""
+    sum of its rows before they are rounded; what is not needed is None.  ``dz`` may be ``dy`` or ``preact``."""
     torch = _torch()
+    if dz is not None or dbias is not None:
+        _outputs_apart(((dz, "dz"), (dbias, "dbias")), ((dy, "dy"), (preact, "preact")), {("dz", "dy"), ("dz", "preact")})
     lib = _cabi.load()
     M, N, dev = _first(dy, "dy")
     act = _act_code(activation)
@@ -358,6 +402,8 @@ def spmm_csr_grad_values(a: DeviceCsr, B, dy, preact=None, activation: Optional[
     ``dz = dy * activation'(preact)`` not rounded in between; float32, one per entry.  For a ``DeviceCsr`` of a slice of
     ``indptr`` the entries count from the slice's first, and what is behind its last is left as it is."""
     torch = _torch()
+    if out is not None:
+        _outputs_apart(((out, "out"),), ((B, "B"), (dy, "dy"), (preact, "preact")))
     K, N, dev = _first(B, "B")
     M = a.shape[0]
     _need(K == a.shape[1], "B must have one row per matrix column")

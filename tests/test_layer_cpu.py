@@ -160,3 +160,62 @@ def test_slopes_by_differences(name):
 def test_transposed_pattern_refusals(indptr, indices, shape):
     with pytest.raises(ValueError):
         layer.CsrTranspose.from_host(np.array(indptr), np.array(indices), shape, "cpu")
+
+
+def views(pitch=32):
+    buf = torch.zeros(40 * pitch + 64)
+    return buf, lambda rows, N, ld, at: torch.as_strided(buf, (rows, N), (ld, 1), at)
+
+
+def by_bytes(a, b):
+    def held(t):
+        return {t.data_ptr() + 4 * (i * t.stride(0) + k) for i in range(t.shape[0]) for k in range(t.shape[1])}
+    return bool(held(a) & held(b))
+
+
+def test_shared_memory_of_rows():
+    """Against the sets of addresses, for rows at one distance and for single rows; equal where rows lie at two distances and
+    apart, or one may be taken to share."""
+    buf, view = views()
+    rng = np.random.default_rng(0)
+    for _ in range(3000):
+        ld = int(rng.integers(1, 33))
+        shapes = [(int(rng.integers(0, 6)), int(rng.integers(1, ld + 1)), ld, int(rng.integers(0, 200))) for _ in range(2)]
+        a, b = (view(*s) for s in shapes)
+        one_step = shapes[0][0] < 2 or shapes[1][0] < 2 or all(s[1] < ld for s in shapes)
+        if one_step:
+            assert layer._share_memory(a, b) == by_bytes(a, b) == layer._share_memory(b, a), shapes
+        else:
+            assert layer._share_memory(a, b) or not by_bytes(a, b), shapes
+    v, w = buf[10:50], buf[49:60]
+    assert layer._share_memory(v, w) and not layer._share_memory(buf[10:49], w) and not layer._share_memory(v, buf[:0])
+
+
+@pytest.mark.parametrize("out, other, refused", [
+    ((4, 8, 8, 16), (20, 8, 8, 0), True),          # rows 2 to 5 of it
+    ((4, 8, 8, 160), (20, 8, 8, 0), False),        # behind it
+    ((20, 8, 32, 8), (20, 8, 32, 0), False),       # columns beside it
+    ((20, 8, 32, 7), (20, 8, 32, 0), True),        # one column in common
+    ((20, 8, 32, 25), (20, 8, 32, 0), True),       # reaches into the next row
+    ((1, 8, 8, 40), (20, 8, 32, 0), False),        # a row in a gap
+    ((20, 8, 8, 0), (20, 8, 8, 8), True),          # the same rows, one further
+    ((4, 8, 16, 0), (4, 8, 32, 0), True)])         # another distance
+def test_outputs_in_inputs_are_refused(out, other, refused):
+    _, view = views()
+    a, b = view(*out), view(*other)
+    if refused:
+        with pytest.raises(ValueError):
+            layer._outputs_apart([(a, "out"), (None, "preact")], [(b, "B"), (None, "bias")], {("out", "B")})
+    else:
+        layer._outputs_apart([(a, "out"), (None, "preact")], [(b, "B"), (None, "bias")])
+
+
+def test_outputs_that_are_an_input_itself():
+    _, view = views()
+    a = view(5, 8, 16, 3)
+    layer._outputs_apart([(a, "out")], [(view(5, 8, 16, 3), "residual")], {("out", "residual")})
+    for given, may_be in (([(a, "out")], ()), ([(a, "out"), (a, "preact")], {("out", "residual")})):
+        with pytest.raises(ValueError):
+            layer._outputs_apart(given, [(a, "residual")], may_be)
+    with pytest.raises(ValueError):
+        layer._outputs_apart([(a, "out")], [(a.view(torch.int32), "residual")], {("out", "residual")})

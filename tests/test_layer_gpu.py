@@ -808,3 +808,61 @@ def test_eight_bit_rows_of_tiny_numbers(cuda_device):
     # 2^-150 * rstd (below 2^-88 here); eps in 32 bits and the square's sum: 2^-20
     off = 2.0 ** -4 * y.abs() * 1.01 + 2.0 ** -10 * s + 2.0 ** -88 + 2.0 ** -20 * y.abs()
     assert bool(((back - y).abs() <= off).all()) and bool((back[4] == 0).all())
+
+
+def test_outputs_in_the_memory_of_inputs_are_refused(cuda_device):
+    M = N = 32
+    p = pattern(M, M, 1)
+    A = csr_on(cuda_device, p, (M, M))
+    T = layer.CsrTranspose.of(A)
+    wide = torch.randn(M + 8, 3 * N, device=cuda_device)
+    B, side, w = wide[:M, :N], wide[:M, N:2 * N], torch.ones(N, device=cuda_device)
+    v = torch.ones(M, device=cuda_device)
+    for f in (lambda: layer.spmm_csr_act(A, B, out=wide[5:25, :N], row_range=(5, 25)),      # rows of B that other rows read
+              lambda: layer.spmm_csr_act(A, B, out=wide[8:, :N]), lambda: layer.spmm_csr_act(A, B, preact=wide[:M, N - 1:2 * N - 1]),
+              lambda: layer.spmm_csr_act(A, B, out=side, preact=side), lambda: layer.spmm_csr_act(A, B, out=side, preact=wide[1:M + 1, N:2 * N]),
+              lambda: layer.spmm_csr_act(A, B, out=side, residual=wide[1:M + 1, N:2 * N]),
+              lambda: layer.spmm_csr_act(A, B, preact=side, residual=wide[1:M + 1, N:2 * N]),
+              lambda: layer.spmm_csr_act(T, B, values=A.data, out=B), lambda: layer.rms_norm(B, w, out=wide[1:M + 1, :N]),
+              lambda: layer.rms_norm(B, w, residual=side, sum_out=side, out=side),
+              lambda: layer.rms_norm(B, w, residual=side, sum_out=wide[2:M + 2, :N]), lambda: layer.rms_norm(B, v, rstd=v),
+              lambda: layer.rms_norm(B, w, out_dtype=E4M3, scale=v, rstd=v), lambda: layer.rms_norm_backward(B, side, w, v, dx=wide[3:M + 3, :N]),
+              lambda: layer.rms_norm_backward(B, side, w, v, dweight=v), lambda: layer.act_backward(B, side, "silu", dz=wide[1:M + 1, :N]),
+              lambda: layer.act_backward(B, side, "silu", dbias=wide[0, :N]),
+              lambda: layer.spmm_csr_grad_values(A, B, side, out=wide.view(-1)[:A.nnz])):
+        with pytest.raises(ValueError, match="lies in the memory of"):
+            f()
+
+
+def test_outputs_beside_or_in_place_of_inputs(cuda_device):
+    """Column slices of one buffer, and the inputs that an output may be, give what separate outputs give."""
+    g = gen(3)
+    for N in (32, 33):
+        M = 70
+        A = csr_on(cuda_device, pattern(M, M, 1, 8.0, 70), (M, M))
+        for dtype in (F32, BF16):
+            wide = torch.randn(M, 3 * N, generator=g).to(dtype).to(cuda_device)
+            B, C, R = (wide[:, i * N:(i + 1) * N] for i in range(3))
+            same = lambda x, y: torch.equal(x, y)
+            want = layer.spmm_csr_act(A, B, activation="gelu", residual=R)
+            assert same(layer.spmm_csr_act(A, B, activation="gelu", residual=R, out=C), want)
+            pre = torch.empty(M, N, dtype=dtype, device=cuda_device)
+            layer.spmm_csr_act(A, B, activation="gelu", preact=pre)
+            res = R.clone()
+            assert same(layer.spmm_csr_act(A, B, activation="gelu", residual=res, preact=res), want) and same(res, pre)
+            w = torch.randn(N, generator=g).to(cuda_device)
+            n = layer.rms_norm(B, w, residual=R)
+            for i in range(2):
+                x, r = B.clone(), R.clone()
+                assert same(layer.rms_norm(x, w, residual=r, out=(x, r)[i]).y, n.y)
+                x, r = B.clone(), R.clone()
+                m = layer.rms_norm(x, w, residual=r, sum_out=(x, r)[i], out=(x, r)[1 - i])
+                assert same(m.y, n.y) and same(m.h, n.h)
+            want = layer.act_backward(B, R, "silu")
+            for i in range(2):
+                x, r = B.clone(), R.clone()
+                assert all(same(*p) for p in zip(layer.act_backward(x, r, "silu", dz=(x, r)[i]), want))
+            want = layer.rms_norm_backward(B, R, w, n.rstd, dh=C)
+            for i in range(3):
+                x, r, c = B.clone(), R.clone(), C.clone()
+                assert all(same(*p) for p in zip(layer.rms_norm_backward(x, r, w, n.rstd, dh=c, dx=(x, r, c)[i]), want))
