@@ -462,12 +462,19 @@ int lf_spmm_csr_act(const int64_t* indptr /*[dev]*/, const int32_t* indices /*[d
                     void* workspace /*[dev]*/, size_t workspace_bytes, void* stream);
 
 /* dz = dy * activation'(preact) (in the type of both; NULL: not wanted) and dbias = the sum of its rows
- * before they are rounded (NULL: not wanted).  preact may be NULL for LF_ACT_NONE. */
+ * before they are rounded (NULL: not wanted).  preact may be NULL for LF_ACT_NONE.  dz may be dy or preact itself.
+ * lf_act_backward_as: dz in dz_dtype, which is dtype or float32 (then not in place of a 16-bit matrix).  Slopes reach
+ * 1.13, and a product with a small one may be smaller than any float16: where A^T dz would still be a number, dz in
+ * float16 may not be. */
 size_t lf_act_backward_workspace_bytes(int64_t rows, int32_t N);
 int lf_act_backward(const void* dy /*[dev]*/, int64_t ld_dy, const void* preact /*[dev]*/, int64_t ld_preact,
                     int32_t dtype, int32_t activation, void* dz /*[dev] out*/, int64_t ld_dz,
                     float* dbias /*[dev] out, N*/, int64_t rows, int32_t N, void* workspace /*[dev]*/,
                     size_t workspace_bytes, void* stream);
+int lf_act_backward_as(const void* dy /*[dev]*/, int64_t ld_dy, const void* preact /*[dev]*/, int64_t ld_preact,
+                       int32_t dtype, int32_t activation, void* dz /*[dev] out*/, int32_t dz_dtype, int64_t ld_dz,
+                       float* dbias /*[dev] out, N*/, int64_t rows, int32_t N, void* workspace /*[dev]*/,
+                       size_t workspace_bytes, void* stream);
 
 /* Gradient of the values: dvalues[e] = <dy[r,:] * activation'(preact[r,:]), B[indices[e],:]> for the
  * entries e of the rows r of [row_begin, row_end), those of value 0 among them, counted from the first; dy and

@@ -120,6 +120,8 @@ SIGNATURES = {
     "lf_act_backward_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int32]),
     "lf_act_backward": (C.c_int, [vp, C.c_int64, vp, C.c_int64, C.c_int32, C.c_int32, vp, C.c_int64, vp, C.c_int64, C.c_int32,
                                   vp, C.c_size_t, vp]),
+    "lf_act_backward_as": (C.c_int, [vp, C.c_int64, vp, C.c_int64, C.c_int32, C.c_int32, vp, C.c_int32, C.c_int64, vp, C.c_int64,
+                                     C.c_int32, vp, C.c_size_t, vp]),
     "lf_spmm_csr_grad_values": (C.c_int, [vp, vp, C.c_int64, C.c_int64, C.c_int64, vp, C.c_int64, vp, C.c_int64, C.c_int32,
                                           C.c_int32, vp, C.c_int32, C.c_int64, C.c_int32, vp, vp]),
     "lf_rms_norm": (C.c_int, [vp, C.c_int32, C.c_int64, vp, C.c_int64, vp, C.c_int64, vp, C.c_int32, C.c_float, vp, C.c_int32,

@@ -25,10 +25,11 @@ struct ActGradArgs {
 // the rows, so that the bias's sum stays in registers.  The inputs are read once and dZ is written once: memory bounds it,
 // and, with the error function's slope, the special functions (2^18 rows of 256 bfloat16, gelu: 91 us, 4.4 TB/s; the bytes
 // alone would take 61).
-template <int DT, int VEC>
+template <int DT, int OUT, int VEC>   // of dy and z, of dz
 __global__ void __launch_bounds__(256)
 act_grad_kernel(ActGradArgs a) {
   using E = typename Type<DT>::T;
+  using O = typename Type<OUT>::T;
   __shared__ float sums[256 * VEC];
   const int t = threadIdx.x % a.per_row, r = threadIdx.x / a.per_row, side = 256 / a.per_row;
   const int f = (blockIdx.y * a.per_row + t) * VEC;
@@ -51,9 +52,9 @@ act_grad_kernel(ActGradArgs a) {
         s[i] += v[i];
       }
       if (a.dz) {
-        Pack<DT, VEC> o;
+        Pack<OUT, VEC> o;
         o.put(v);
-        o.keep(reinterpret_cast<E*>(a.dz) + row * a.ld_dz + f);   // gathered next
+        o.keep(reinterpret_cast<O*>(a.dz) + row * a.ld_dz + f);   // gathered next
       }
     }
   }
@@ -285,8 +286,16 @@ size_t lf_act_backward_workspace_bytes(int64_t rows, int32_t N) {
 int lf_act_backward(const void* dy, int64_t ld_dy, const void* preact, int64_t ld_preact, int32_t dtype,
                     int32_t activation, void* dz, int64_t ld_dz, float* dbias, int64_t rows, int32_t N,
                     void* workspace, size_t workspace_bytes, void* stream) {
+  return lf_act_backward_as(dy, ld_dy, preact, ld_preact, dtype, activation, dz, dtype, ld_dz, dbias, rows, N, workspace,
+                            workspace_bytes, stream);
+}
+
+int lf_act_backward_as(const void* dy, int64_t ld_dy, const void* preact, int64_t ld_preact, int32_t dtype,
+                       int32_t activation, void* dz, int32_t dz_dtype, int64_t ld_dz, float* dbias, int64_t rows,
+                       int32_t N, void* workspace, size_t workspace_bytes, void* stream) {
   LF_REQUIRE(rows >= 0 && rows < (1ll << 31) - 64 && N >= 1, "bad sizes");
   LF_REQUIRE(is_wide_dtype(dtype), "the type must be float32, bfloat16 or float16");
+  LF_REQUIRE(!dz || dz_dtype == dtype || dz_dtype == LF_DTYPE_F32, "dz must have dy's type or float32");
   LF_REQUIRE(activation >= LF_ACT_NONE && activation <= LF_ACT_GELU_TANH, "unknown activation");
   LF_REQUIRE(dz || dbias, "nothing to compute");
   cudaStream_t st = (cudaStream_t)stream;
@@ -301,7 +310,7 @@ int lf_act_backward(const void* dy, int64_t ld_dy, const void* preact, int64_t l
                 lf_act_backward_workspace_bytes(rows, N));
   const void* z = activation == LF_ACT_NONE ? nullptr : preact;
   const int per = 16 / dtype_bytes(dtype);
-  const bool vec = N % per == 0 && on_grid16(dy, ld_dy, dtype) && (!z || on_grid16(z, ld_preact, dtype)) && (!dz || on_grid16(dz, ld_dz, dtype));
+  const bool vec = N % per == 0 && on_grid16(dy, ld_dy, dtype) && (!z || on_grid16(z, ld_preact, dtype)) && (!dz || on_grid16(dz, ld_dz, dz_dtype));
   const int pieces = vec ? N / per : N;
   int per_row = 4;
   while (per_row < pieces && per_row < 256) per_row *= 2;
@@ -310,10 +319,15 @@ int lf_act_backward(const void* dy, int64_t ld_dy, const void* preact, int64_t l
   const int parts = (int)(want < kMostParts ? want : kMostParts);
   const dim3 grid((unsigned)parts, (unsigned)((pieces + per_row - 1) / per_row));
   LF_REQUIRE(grid.y < 65536, "too many features");
-#define LF_GO(DT_, VEC_) act_grad_kernel<DT_, VEC_><<<grid, 256, 0, st>>>(a)
-  if (dtype == LF_DTYPE_F32) { if (vec) LF_GO(LF_DTYPE_F32, 4); else LF_GO(LF_DTYPE_F32, 1); }
-  else if (dtype == LF_DTYPE_BF16) { if (vec) LF_GO(LF_DTYPE_BF16, 8); else LF_GO(LF_DTYPE_BF16, 1); }
-  else { if (vec) LF_GO(LF_DTYPE_F16, 8); else LF_GO(LF_DTYPE_F16, 1); }
+  const bool wide = dz && dz_dtype != dtype;
+#define LF_GO(DT_, OUT_, VEC_) \
+  if (vec) act_grad_kernel<DT_, OUT_, VEC_><<<grid, 256, 0, st>>>(a); \
+  else act_grad_kernel<DT_, OUT_, 1><<<grid, 256, 0, st>>>(a)
+  if (dtype == LF_DTYPE_F32) { LF_GO(LF_DTYPE_F32, LF_DTYPE_F32, 4); }
+  else if (dtype == LF_DTYPE_BF16 && !wide) { LF_GO(LF_DTYPE_BF16, LF_DTYPE_BF16, 8); }
+  else if (dtype == LF_DTYPE_BF16) { LF_GO(LF_DTYPE_BF16, LF_DTYPE_F32, 8); }
+  else if (!wide) { LF_GO(LF_DTYPE_F16, LF_DTYPE_F16, 8); }
+  else { LF_GO(LF_DTYPE_F16, LF_DTYPE_F32, 8); }
 #undef LF_GO
   LF_CUDA_CHECK(cudaGetLastError());
   if (dbias) LF_CUDA_CHECK(launch_column_sum(a.partial, parts, N, dbias, st));

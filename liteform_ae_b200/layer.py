@@ -368,9 +368,10 @@ def spmm_csr_act(a, B, scale=None, bias=None, activation: Optional[str] = None, 
 
 
 def act_backward(dy, preact=None, activation: Optional[str] = None, dz=None, need_dz: bool = True, need_dbias: bool = True,
-                 dbias=None, workspace: Optional[Workspace] = None):
-    """``lf_act_backward``: ``(dz, dbias)`` with ``dz = dy * activation'(preact)`` in dy's type and ``dbias`` the float32
-    sum of its rows before they are rounded; what is not needed is None.  ``dz`` may be ``dy`` or ``preact``."""
+                 dbias=None, workspace: Optional[Workspace] = None, dz_dtype=None):
+    """``lf_act_backward_as``: ``(dz, dbias)`` with ``dz = dy * activation'(preact)`` in ``dz_dtype`` (dy's, the default, or
+    float32) and ``dbias`` the float32 sum of its rows before they are rounded; what is not needed is None.  ``dz`` may be
+    ``dy`` or ``preact``."""
     torch = _torch()
     if dz is not None or dbias is not None:
         _outputs_apart(((dz, "dz"), (dbias, "dbias")), ((dy, "dy"), (preact, "preact")), {("dz", "dy"), ("dz", "preact")})
@@ -381,19 +382,21 @@ def act_backward(dy, preact=None, activation: Optional[str] = None, dz=None, nee
     if act != _cabi.LF_ACT_NONE:
         _need(preact is not None and preact.dtype == dy.dtype, "preact must be given, in dy's type")
         ld_z = _matrix(preact, "preact", M, N, dev)
+    if dz_dtype is None:
+        dz_dtype = dy.dtype if dz is None else dz.dtype
     if dz is None and need_dz:
-        dz = _rows_like(dy, dy.dtype)
+        dz = _rows_like(dy, dz_dtype)
     if dbias is None and need_dbias:
         dbias = torch.empty(N, dtype=torch.float32, device=dy.device)
     _need(dz is not None or dbias is not None, "nothing to compute")
-    _need(dz is None or dz.dtype == dy.dtype, "dz must have dy's type")
+    _need(dz is None or (dz.dtype == dz_dtype and dz_dtype in (dy.dtype, torch.float32)), "dz must have dz_dtype: dy's type or float32")
     ld_dz = 0 if dz is None else _matrix(dz, "dz", M, N, dev)
     b_ptr = 0 if dbias is None else _vector(dbias, "dbias", N, dev, torch.float32)
     nbytes = 0 if dbias is None else lib.lf_act_backward_workspace_bytes(M, N)
     keep, ws, nws = _scratch(nbytes, workspace, dy)
     call = (dy.data_ptr(), ld_dy, 0 if act == _cabi.LF_ACT_NONE else preact.data_ptr(), ld_z, code, act,
-            0 if dz is None else dz.data_ptr(), ld_dz, b_ptr, M, N, ws, nws, stream_of(dev))
-    _run(lib.lf_act_backward, call, dev)
+            0 if dz is None else dz.data_ptr(), code if dz is None else _code(dz_dtype), ld_dz, b_ptr, M, N, ws, nws, stream_of(dev))
+    _run(lib.lf_act_backward_as, call, dev)
     return dz, dbias
 
 
@@ -430,11 +433,13 @@ class ActGradients(NamedTuple):
 
 
 def spmm_csr_act_backward(a: DeviceCsr, a_t: Optional[CsrTranspose], B, dy, preact=None, activation: Optional[str] = None,
-                          need=("dB", "dvalues", "dbias"), workspace: Optional[Workspace] = None) -> ActGradients:
+                          need=("dB", "dvalues", "dbias"), workspace: Optional[Workspace] = None, dz_dtype=None) -> ActGradients:
     """Gradients of ``spmm_csr_act(a, B, bias=..., activation=..., preact=...)`` from ``dy``, the gradient of its result
     (which is also that of the residual): ``act_backward``, ``A^T @ dz`` and ``spmm_csr_grad_values``.  ``preact`` and dy
     have one type, 16 or 32 bits like B (8-bit rows have no gradient here); ``need`` names the ones wanted, ``a_t`` is
-    used for dB only.  dz is rounded to dy's type for dB; dvalues and dbias take it unrounded."""
+    used for dB only.  dB is made of dz rounded to ``dz_dtype``, dy's type or float32; dvalues and dbias take it unrounded.
+    The default is dy's type, except for float16 and an activation with slopes beside 0 and 1: there dz may pass 65504 or
+    vanish where dB would not, so it is float32 (twice the bytes gathered)."""
     unknown = set(need) - {"dB", "dvalues", "dbias"}
     _need(not unknown, "need names dB, dvalues and dbias")
     _code(B.dtype)
@@ -444,8 +449,11 @@ def spmm_csr_act_backward(a: DeviceCsr, a_t: Optional[CsrTranspose], B, dy, prea
     _need("dB" not in need or (a_t is not None and a_t.shape == (a.shape[1], a.shape[0]) and a_t.nnz == a.nnz),
           "dB needs the transposed pattern of a")
     want_dz = "dB" in need and not plain
+    if dz_dtype is None and dy.dtype == _torch().float16 and activation != "relu":
+        dz_dtype = _torch().float32
     if want_dz or "dbias" in need:
-        got, dbias = act_backward(dy, preact, activation, need_dz=want_dz, need_dbias="dbias" in need, workspace=workspace)
+        got, dbias = act_backward(dy, preact, activation, need_dz=want_dz, need_dbias="dbias" in need, workspace=workspace,
+                                  dz_dtype=dz_dtype if want_dz else None)
         dz = got if want_dz else dy
     if "dB" in need:
         dB = spmm_csr_act(a_t, dz, values=a.data, out_dtype=B.dtype, workspace=workspace)

@@ -219,3 +219,19 @@ def test_outputs_that_are_an_input_itself():
             layer._outputs_apart(given, [(a, "residual")], may_be)
     with pytest.raises(ValueError):
         layer._outputs_apart([(a, "out")], [(a.view(torch.int32), "residual")], {("out", "residual")})
+
+
+def act_grad_as(**kw):
+    a = dict(dy=P, ld_dy=8, z=P, ld_z=8, dtype=BF16, act=_cabi.LF_ACT_SILU, dz=P, dzd=F32, ld_dz=8, db=P, rows=2, N=8, ws=P, nws=1 << 20)
+    a.update(kw)
+    return _cabi.load().lf_act_backward_as(*a.values(), 0)
+
+
+@pytest.mark.parametrize("kw", [dict(dzd=_cabi.LF_DTYPE_F16), dict(dtype=F32, dzd=BF16), dict(dzd=E4M3), dict(dzd=9), dict(ld_dz=7), dict(N=0),
+                                dict(rows=-1), dict(dtype=E4M3), dict(act=9), dict(dz=0, db=0), dict(dy=0), dict(z=0)])
+def test_act_backward_as_refusals(kw):
+    assert act_grad_as(**kw) == BAD
+
+
+def test_act_backward_as_workspace():
+    assert act_grad_as(nws=0) == SMALL and act_grad_as(rows=0, db=0, dy=0, z=0, ws=0, nws=0) == 0

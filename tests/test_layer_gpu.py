@@ -866,3 +866,49 @@ def test_outputs_beside_or_in_place_of_inputs(cuda_device):
             for i in range(3):
                 x, r, c = B.clone(), R.clone(), C.clone()
                 assert all(same(*p) for p in zip(layer.rms_norm_backward(x, r, w, n.rstd, dh=c, dx=(x, r, c)[i]), want))
+
+
+@pytest.mark.parametrize("name", ref.ACTS)
+@pytest.mark.parametrize("N", [16, 21])
+def test_gradient_of_float16_beyond_its_range(cuda_device, name, N):
+    """dz beyond 65504, and below the smallest float16, where dB is an ordinary number: A's values bring it back."""
+    g = gen(N)
+    M, K = 64, 48
+    indptr, indices, vals = pattern(M, K, 6, 8.0)
+    dyv = torch.randn(M, N, generator=g)
+    dyv[::2] = torch.sign(dyv[::2]) * 65000.0
+    dyv[1::2] *= 2.0 ** -24
+    vals *= torch.repeat_interleave(torch.tensor([2.0 ** -18, 2.0 ** 20]).repeat(M // 2), torch.diff(indptr))
+    zv = (1.5 + torch.rand(M, N, generator=g)).half().double()      # where the slopes of silu and gelu are above 1
+    zv[1::2] -= 5
+    A = csr_on(cuda_device, (indptr, indices, vals), (M, K))
+    B, _, Bv = features(K, N, F16, g, cuda_device)
+    dy, z = dyv.half().to(cuda_device), zv.half().to(cuda_device)
+    got = layer.spmm_csr_act_backward(A, layer.CsrTranspose.of(A), B, dy, preact=z, activation=name)
+    dz_dtype = F16 if name in ("none", "relu") else F32
+    _, _, dB, dBoff, _, _, db, dboff = gradients64(ref.dense(indptr, indices, vals, (M, K)), Bv, dyv.half().double(), zv, name, dz_dtype)
+    assert float(dB.abs().max()) < 6e4
+    ref.close(got.dB, dB, ref.rounded(dB, dBoff, F16), name)
+    ref.close(got.dbias, db, dboff + ref.TINY[F32], name)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("N,pitch,shift", [(64, 64, 0), (64, 72, 4), (31, 33, 2), (300, 300, 0)])
+def test_act_backward_into_float32(cuda_device, dtype, N, pitch, shift):
+    g, M = gen(N), 90
+    dy, dyv = rows_of((M, N), dtype, g, cuda_device, N + 1)
+    z, zv = rows_of((M, N), dtype, g, cuda_device)
+    for name in ref.ACTS:
+        buf = torch.full((M * pitch + shift + 8,), 3.0, device=cuda_device)
+        dz = torch.as_strided(buf, (M, N), (pitch, 1), shift)
+        want = dyv * (ref.slope(zv, name) if name != "none" else 1)
+        off = (0 if name in ("none", "relu") else ref.SLOPE_ERROR) * (1 + zv.abs()) * dyv.abs() + 2 * U32 * want.abs()
+        got, db = layer.act_backward(dy, z, name, dz=dz)
+        assert got is dz
+        ref.close(dz, want, off, name)
+        assert torch.equal(layer.act_backward(dy, z, name, dz_dtype=F32)[0], dz) and bool((buf[:shift] == 3).all())
+        assert torch.equal(layer.act_backward(dy, z, name, need_dz=False)[1], db)
+    for f in (lambda: layer.act_backward(dy, z, "silu", dz_dtype=F16 if dtype == BF16 else BF16), lambda: layer.act_backward(dy, z, "silu", dz=dz, dz_dtype=dtype),
+              lambda: layer.act_backward(dz, dz.clone(), "silu", dz_dtype=dtype), lambda: layer.act_backward(dy, z, "silu", dz_dtype=E4M3)):
+        with pytest.raises(ValueError):
+            f()
