@@ -45,7 +45,7 @@ __device__ __forceinline__ char* row_at(const void* base, int row, uint32_t pitc
 // first on to the row's end.  vec: the row is on the 16-byte grid and holds whole eights, so blocks move as they are, and
 // `w` holds them side by side; otherwise one by one, one a word.  (In a loop over memory, as each is needed once: 80 802 rows with 1.3 M
 // entries, 168 features in 8 bits, 326 us for 130.)
-template <int BLOCKS, int n>
+template <int BLOCKS, int n, bool FULL>   // FULL: activations for results in 32 bits
 struct RowIo {
   static __device__ __forceinline__ void load(const char* p, int dt, bool vec, int apart, int left, uint32_t* w) {
     if (vec) {
@@ -115,7 +115,7 @@ struct RowIo {
     }
     const int at = f * dtype_bytes(c_dtype);
     if (a.preact) store(row_at(a.preact, row, a.pitch_pre) + at, c_dtype, vec, apart, left, z);
-    activate_all<BLOCKS * n>(z, a.act);
+    activate_all<BLOCKS * n, FULL>(z, a.act);
     if (a.residual) add(w, res_dtype, vec, z);
     store(row_at(a.C, row, a.pitch_c) + at, c_dtype, vec, apart, left, z);
   }
@@ -123,8 +123,8 @@ struct RowIo {
 // eight features, the residual fetched here
 __device__ __forceinline__ void finish8(const ActArgs& a, int row, int f, const float* bias, float* z) {
   __align__(16) uint32_t w[8];
-  if (a.residual) RowIo<1, 8>::load(row_at(a.residual, row, a.pitch_res) + f * dtype_bytes(a.res_dtype), a.res_dtype, a.vec, 8, a.N - f, w);
-  RowIo<1, 8>::finish(a, a.c_dtype, a.res_dtype, a.vec, row, f, 8, a.N - f, bias, w, z);
+  if (a.residual) RowIo<1, 8, true>::load(row_at(a.residual, row, a.pitch_res) + f * dtype_bytes(a.res_dtype), a.res_dtype, a.vec, 8, a.N - f, w);
+  RowIo<1, 8, true>::finish(a, a.c_dtype, a.res_dtype, a.vec, row, f, 8, a.N - f, bias, w, z);
 }
 
 // ---- the walk ---------------------------------------------------------------------------------------
@@ -141,7 +141,7 @@ struct ActWork {
   // the lane's share of a row in memory
   static constexpr int kBlock = S::kShifted ? 1 : S::VEC < 8 ? S::VEC : 8, kBlocks = S::kFloats / kBlock;   // whole blocks in a row of whole eights
   static constexpr int kApart = S::kShifted ? G : S::VEC > 8 ? 8 : G * S::VEC;
-  using Io = RowIo<kBlocks, kBlock>;
+  using Io = RowIo<kBlocks, kBlock, IO != kTyped || kOwn<DT> == LF_DTYPE_F32>;
   const ActArgs& a;
   const float* bias;    // in shared memory, from the lane's first feature on
   int64_t slots;        // of the range in `partial`

@@ -45,7 +45,7 @@ act_grad_kernel(ActGradArgs a) {
       float v[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) v[i] = a.z ? z.get(i) : 0.f;
-      if (a.z) slopes<VEC>(v, a.act);
+      if (a.z) slopes<VEC, DT == LF_DTYPE_F32>(v, a.act);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         v[i] = a.z ? d.get(i) * v[i] : d.get(i);
@@ -173,7 +173,7 @@ struct GradWork {
       float z[S::kFloats];
       load(row, d, z);
       if (a.z) {
-        slopes<S::kFloats>(z, a.act);
+        slopes<S::kFloats, !VIO || DT == LF_DTYPE_F32>(z, a.act);
 #pragma unroll
         for (int i = 0; i < S::kFloats; ++i) d[i] *= z[i];
       }

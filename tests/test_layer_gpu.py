@@ -1,4 +1,6 @@
 """The layer operators on the GPU against plain 64-bit forms."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -912,3 +914,41 @@ def test_act_backward_into_float32(cuda_device, dtype, N, pitch, shift):
               lambda: layer.act_backward(dz, dz.clone(), "silu", dz_dtype=dtype), lambda: layer.act_backward(dy, z, "silu", dz_dtype=E4M3)):
         with pytest.raises(ValueError):
             f()
+
+
+# Relative bounds of the activations, in units of U = 2^-24.  silu: expf and the reciprocal are off by a unit in the last place (2 U)
+# each, 1 + p, p r and the product with z by U: 7 U; in 16 bits 2^x by 4 U, its argument by a rounded constant and product, 1.5 |u| U.
+# gelu_tanh: 4 roundings in u add 4 |u| U.  gelu: the series is off by 2.9e-7 (5 U), the reciprocal's other half unit counts
+# 2.6-fold, 2^x is off by 4 U, three products by 3 U: 16 U; three roundings in the exponent z^2 / 2 add 1.5 z^2 U.  Slopes add two
+# terms with 3 more roundings; in 16 bits s (1 - s) is off by U of s where s is near 1.
+def activation_forms(z, name, dtype):
+    """(value, slope's two terms, relative bound), all accurate in the lower tail."""
+    if name == "gelu":
+        phi, c = torch.exp(-z * z / 2) / math.sqrt(2 * math.pi), torch.special.erfc(-z * math.sqrt(0.5)) / 2
+        return z * c, (c, z * phi), (16 + 1.5 * z * z) * U32
+    k0, k1 = (1.0, 0.0) if name == "silu" else (2 * math.sqrt(2 / math.pi), 0.044715)
+    u = k0 * z * (1 + k1 * z * z)
+    s, d = torch.special.expit(u), torch.special.expit(u) * torch.special.expit(-u)
+    off = 8 + (4 * u.abs() if name == "gelu_tanh" else 0) + (0 if dtype == F32 else 2 + 1.5 * u.abs())
+    return z * s, (s, z * d * k0 * (1 + 3 * k1 * z * z)), off * U32
+
+
+@pytest.mark.parametrize("name", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_tails_of_the_activations(cuda_device, name, dtype):
+    """For z in [-9, 9], relative to the results themselves: a tail that is lost, or known to an absolute error, fails."""
+    z = torch.linspace(-9, 9, 8192).to(dtype)
+    N, dev = len(z), cuda_device
+    A = hyb.DeviceCsr(torch.tensor([0, 1, 1], device=dev), torch.zeros(1, dtype=torch.int32, device=dev), None, (2, 1))
+    want, (s, t), off = activation_forms(z.double(), name, dtype)
+    B = z[None].to(dev)
+    ref.close(layer.spmm_csr_act(A, B, activation=name)[0], want, ref.rounded(want, off * want.abs(), dtype), name)
+    ref.close(layer.spmm_csr_act(A, B * 0, bias=B[0], activation=name)[1], want, ref.rounded(want, off * want.abs(), dtype), name + " of a bias")
+    slope, off = s + t, (off + 3 * U32) * (s + t.abs()) + (0 if dtype == F32 else U32 * t.abs() / (1 - s).clamp(min=U32))
+    one = torch.ones_like(B)
+    ref.close(layer.act_backward(one, B, name, need_dbias=False)[0][0], slope, ref.rounded(slope, off, dtype), name + " slope")
+    unit = torch.zeros_like(B)      # one column at a time, unrounded: the slope times 1
+    for i in range(0, N, 1024):
+        unit.zero_()[0, i] = 1
+        dv = layer.spmm_csr_grad_values(A, B * 0 + 1, torch.cat([unit, unit]), torch.cat([B, B]), name)
+        ref.close(dv, slope[i:i + 1], off[i:i + 1] + ref.TINY[F32], name + " value gradient")
