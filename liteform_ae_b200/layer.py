@@ -89,18 +89,18 @@ def _first(t, name):
 
 
 def _extent(t):
-    """``(address, bytes of a row, bytes from a row to the next, rows)``; dense tensors count as one row."""
-    e = t.element_size()
-    if t.dim() != 2 or t.shape[0] < 2 or t.stride(0) == t.shape[1]:
-        return t.data_ptr(), t.numel() * e, 0, 1 if t.numel() else 0
-    return t.data_ptr(), t.shape[1] * e, t.stride(0) * e, t.shape[0]
+    """``(address, end, bytes of a row, bytes from a row to the next)``; dense tensors count as one row, at distance 0."""
+    p, e, n = t.data_ptr(), t.element_size(), t.numel()
+    if not n or t.is_contiguous() or t.dim() != 2 or t.shape[0] < 2:
+        return p, p + n * e, n * e, 0
+    step, wide = t.stride(0) * e, t.shape[1] * e
+    return p, p + (t.shape[0] - 1) * step + wide, wide, step
 
 
-def _share_memory(a, b) -> bool:
-    """Whether two matrices or vectors have bytes in common.  Rows at one distance may lie beside each other, as column slices of a
-    buffer do; at two distances, one reaching into the other counts as sharing."""
-    (p, wide_a, step_a, n_a), (q, wide_b, step_b, n_b) = _extent(a), _extent(b)
-    if not n_a or not n_b or p + (n_a - 1) * step_a + wide_a <= q or q + (n_b - 1) * step_b + wide_b <= p:
+def _extents_share(a, b) -> bool:
+    p, end_a, wide_a, step_a = a
+    q, end_b, wide_b, step_b = b
+    if end_a <= q or end_b <= p or p == end_a or q == end_b:
         return False
     step = step_a or step_b
     if not step or (step_a and step_b and step_a != step_b):
@@ -109,15 +109,25 @@ def _share_memory(a, b) -> bool:
     return gap < wide_a or gap + wide_b > step
 
 
+def _share_memory(a, b) -> bool:
+    """Whether two matrices or vectors have bytes in common.  Rows at one distance may lie beside each other, as column slices of a
+    buffer do; at two distances, one reaching into the other counts as sharing."""
+    return _extents_share(_extent(a), _extent(b))
+
+
 def _outputs_apart(given, inputs, may_be=()):
     """Refuses outputs that the caller gave in memory that the call reads or writes elsewhere: ``given`` and ``inputs`` are
     ``(tensor, name)``, tensors may be None; ``may_be``: pairs of names that may be one and the same matrix."""
-    given = [(t, name) for t, name in given if t is not None]
-    for i, (t, name) in enumerate(given):
-        for other, of in given[i + 1:] + [o for o in inputs if o[0] is not None]:
-            if _share_memory(t, other) and not ((name, of) in may_be and t.data_ptr() == other.data_ptr() and t.dtype == other.dtype
-                                                and t.shape == other.shape and t.stride() == other.stride()):
+    seen = [(t, name, _extent(t)) for t, name in inputs if t is not None]
+    for t, name in given:
+        if t is None:
+            continue
+        at = _extent(t)
+        for other, of, there in seen:
+            if at[0] < there[1] and there[0] < at[1] and _extents_share(at, there) and not (
+                    (name, of) in may_be and at[0] == there[0] and t.dtype == other.dtype and t.shape == other.shape and t.stride() == other.stride()):
                 raise ValueError(f"{name} lies in the memory of {of}")
+        seen.append((t, name, at))
 
 
 def _act_code(activation):
@@ -187,7 +197,7 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, out_dtype=None, out=No
     if out is not None or sum_out is not None or scale is not None or rstd is not None:
         _outputs_apart(((out, "out"), (sum_out, "sum_out"), (scale, "scale"), (rstd, "rstd")),
                        ((x, "x"), (residual, "residual"), (weight, "weight")),
-                       {("out", "x"), ("out", "residual"), ("sum_out", "x"), ("sum_out", "residual")})
+                       (("out", "x"), ("out", "residual"), ("sum_out", "x"), ("sum_out", "residual")))
     M, N, dev = _first(x, "x")
     code = _code(x.dtype)
     ld_x = _matrix(x, "x", M, N, dev)
@@ -232,7 +242,7 @@ def rms_norm_backward(dy, h, weight, rstd, dh=None, dx=None, dweight=None, works
     torch = _torch()
     if dx is not None or dweight is not None:
         _outputs_apart(((dx, "dx"), (dweight, "dweight")), ((dy, "dy"), (h, "h"), (dh, "dh"), (weight, "weight"), (rstd, "rstd")),
-                       {("dx", "dy"), ("dx", "h"), ("dx", "dh"), ("dweight", "weight")})
+                       (("dx", "dy"), ("dx", "h"), ("dx", "dh"), ("dweight", "weight")))
     lib = _cabi.load()
     M, N, dev = _first(dy, "dy")
     code = _code(dy.dtype)
@@ -327,7 +337,7 @@ def spmm_csr_act(a, B, scale=None, bias=None, activation: Optional[str] = None, 
     torch = _torch()
     if out is not None or preact is not None:
         _outputs_apart(((out, "out"), (preact, "preact")), ((B, "B"), (residual, "residual"), (bias, "bias"), (scale, "scale")),
-                       {("out", "residual"), ("preact", "residual")})
+                       (("out", "residual"), ("preact", "residual")))
     lib = _cabi.load()
     K, N, dev = _first(B, "B")
     _need(K == a.shape[1], "B must have one row per matrix column")
@@ -374,7 +384,7 @@ def act_backward(dy, preact=None, activation: Optional[str] = None, dz=None, nee
     ``dy`` or ``preact``."""
     torch = _torch()
     if dz is not None or dbias is not None:
-        _outputs_apart(((dz, "dz"), (dbias, "dbias")), ((dy, "dy"), (preact, "preact")), {("dz", "dy"), ("dz", "preact")})
+        _outputs_apart(((dz, "dz"), (dbias, "dbias")), ((dy, "dy"), (preact, "preact")), (("dz", "dy"), ("dz", "preact")))
     lib = _cabi.load()
     M, N, dev = _first(dy, "dy")
     act = _act_code(activation)
