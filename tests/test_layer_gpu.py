@@ -952,3 +952,50 @@ def test_tails_of_the_activations(cuda_device, name, dtype):
         unit.zero_()[0, i] = 1
         dv = layer.spmm_csr_grad_values(A, B * 0 + 1, torch.cat([unit, unit]), torch.cat([B, B]), name)
         ref.close(dv, slope[i:i + 1], off[i:i + 1] + ref.TINY[F32], name + " value gradient")
+
+
+# ---- more rows than a launch has places for: every thread takes several, the last turn is ragged -------
+# (148 * 12 blocks of 256 threads or 148 * 6 of 512 forward, 148 * 3 or 148 blocks backward, 148 * 6 for dz)
+@pytest.mark.parametrize("M,N,extra", [(2000, 4096, 0), (1000, 8192, 8), (20001, 512, 0), (120001, 32, 8), (60001, 47, 1), (30001, 96, 5),
+                                       (1900, 1030, 0), (1001, 4097, 1), (2111, 264, 8)])
+@pytest.mark.parametrize("dtype,out", [(BF16, E4M3), (F32, F32)])
+@pytest.mark.parametrize("form", ["x", "x + r", "into x", "into r"])
+def test_norm_of_many_rows(cuda_device, M, N, extra, dtype, out, form):
+    g = gen(N)
+    x, xv = rows_of((M, N), dtype, g, cuda_device, N + extra)
+    r, rv = (None, None) if form == "x" else rows_of((M, N), dtype, g, cuda_device, N + extra)
+    w = (1 + 0.1 * torch.randn(N, generator=g)).to(dtype).to(cuda_device)
+    n = layer.rms_norm(x, w, residual=r, eps=1e-5, out_dtype=out, sum_out={"into x": x, "into r": r}.get(form))
+    check_norm(x, r, w, 1e-5, n, xv, rv, w.cpu().double())
+
+
+@pytest.mark.parametrize("M,N,extra", [(5000, 512, 0), (1000, 4096, 8), (1000, 20001, 0), (40001, 64, 8), (9000, 47, 1), (700, 8192, 0), (3001, 1030, 2),
+                                       (2000, 264, 0), (500, 2056, 0)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("form", ["plain", "dh", "in place"])
+def test_norm_backward_of_many_rows(cuda_device, M, N, extra, dtype, form):
+    g = gen(M + N)
+    dy, dyv = rows_of((M, N), dtype, g, cuda_device, N + extra)
+    h, hv = rows_of((M, N), dtype, g, cuda_device, N + extra)
+    dh, dhv = (None, None) if form == "plain" else rows_of((M, N), dtype, g, cuda_device, N + extra)
+    w = (1 + 0.1 * torch.randn(N, generator=g)).to(dtype).to(cuda_device)
+    rstd = (hv.square().mean(1) + 1e-6).rsqrt().float().to(cuda_device)
+    dx, dw = layer.rms_norm_backward(dy, h, w, rstd, dh=dh, dx=dy if form == "in place" else None)
+    want, off, dwv, dwoff = norm_grad64(dyv, hv, w.cpu().double(), rstd.cpu().double(), dhv)
+    ref.close(dx, want, ref.rounded(want, off, dtype), "dx")
+    ref.close(dw, dwv, dwoff + ref.TINY[F32], "dw")
+
+
+@pytest.mark.parametrize("M,N,extra", [(3000, 1030, 0), (100_000, 16, 0), (100_001, 17, 2), (40_000, 64, 8), (1500, 5000, 0)])
+@pytest.mark.parametrize("dtype,out", [(F32, F32), (BF16, BF16), (F16, F32)])
+@pytest.mark.parametrize("name", ["none", "silu", "gelu"])
+def test_act_backward_of_many_rows(cuda_device, M, N, extra, dtype, out, name):
+    g = gen(M)
+    dy, dyv = rows_of((M, N), dtype, g, cuda_device, N + extra)
+    z, zv = rows_of((M, N), dtype, g, cuda_device, N)
+    s = ref.slope(zv, name) if name != "none" else torch.ones_like(zv)
+    want = dyv * s
+    off = (ref.SLOPE_ERROR * (1 + zv.abs()) * dyv.abs() if name != "none" else 0) + 2 * U32 * want.abs()
+    dz, db = layer.act_backward(dy, z, name, dz_dtype=out)
+    ref.close(dz, want, ref.rounded(want, off, out), "dz")
+    ref.close(db, want.sum(0), off.sum(0) + (M + 2) * U32 * (want.abs() + off).sum(0) + ref.TINY[F32], "dbias")
