@@ -196,7 +196,11 @@ class MTX:
         return self.csr_host().nnz != self.coo_mtx.nnz
 
     def csr_device(self, device="cuda"):
+        import torch
         from .hyb import DeviceCsr
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:      # the cache is by GPU, whichever is current later
+            device = torch.device("cuda", torch.cuda.current_device())
         key = str(device)
         hit = self._dev_cache.get(key)
         if hit is None or hit[0] != id(self.coo_mtx):

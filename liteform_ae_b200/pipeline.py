@@ -152,18 +152,21 @@ def run_matrix(g: MTX, clf_selection, clf_partition=None, feat_sizes: Iterable[i
     return rows
 
 
-def infer(g: MTX, x, layers: Sequence[dict], eight_bits: bool = True, eps: float = 1e-6, device="cuda"):
+def infer(g: MTX, x, layers: Sequence[dict], eight_bits: bool = True, eps: float = 1e-6, device=None):
     """``x`` (a matrix of 16- or 32-bit features, one row per column of the square matrix ``g``) through layers
 
         h = h + y;   f = rms_norm(h) * norm;   y = activation(A @ f + bias)
 
     starting from h = x and y = 0; returns the last h + y, in x's type.  A layer is a dict with ``norm`` (one weight
     per feature) and optionally ``bias`` and ``activation`` (``layer.ACTIVATIONS``).  ``eight_bits``: the rows that
-    the product gathers are e4m3 with a scale each, a quarter of float32's bytes; otherwise x's type.  Nothing is
-    synchronised, and the matrix is uploaded once."""
+    the product gathers are e4m3 with a scale each, a quarter of float32's bytes; otherwise x's type.  The matrix goes
+    to x's device (``device``, if given, has to be that one) on the first call, which uploads and checks it and waits for
+    that; later calls wait for nothing."""
     import torch
     from . import layer
-    csr = g.csr_device(device)
+    if not x.is_cuda:
+        raise ValueError("x must be a matrix on a CUDA device")
+    csr = g.csr_device(x.device if device is None else device)
     if csr.shape[0] != csr.shape[1]:
         raise ValueError("the matrix must be square")
     if not layers:

@@ -235,3 +235,40 @@ def test_act_backward_as_refusals(kw):
 
 def test_act_backward_as_workspace():
     assert act_grad_as(nws=0) == SMALL and act_grad_as(rows=0, db=0, dy=0, z=0, ws=0, nws=0) == 0
+
+
+def test_matrices_are_kept_by_gpu(monkeypatch):
+    """A matrix uploaded while one GPU is current is not handed out for another."""
+    import scipy.sparse as sp
+    from liteform_ae_b200 import hyb
+    from liteform_ae_b200.format_matrix_market import MTX
+    m = sp.csr_matrix(np.eye(3, dtype=np.float32))
+    g = MTX.from_csr(m.indptr, m.indices, m.data, m.shape, "t")
+    made, current = [], [0]
+    monkeypatch.setattr(hyb.DeviceCsr, "from_host", staticmethod(lambda *a: made.append(str(a[4])) or (str(a[4]), len(made))))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    first = g.csr_device()
+    current[0] = 1
+    second = g.csr_device()
+    assert first[0] == "cuda:0" and second[0] == "cuda:1"
+    assert g.csr_device("cuda:0") is first and g.csr_device(torch.device("cuda", 1)) is second and g.csr_device("cuda") is second
+    assert made == ["cuda:0", "cuda:1"]
+
+
+def test_infer_takes_the_matrix_to_its_rows(monkeypatch):
+    from liteform_ae_b200 import pipeline
+
+    class Stop(Exception):
+        pass
+
+    class Rows:
+        is_cuda, device = True, torch.device("cuda", 3)
+
+    class Matrix:
+        def csr_device(self, device):
+            raise Stop(str(device))
+
+    with pytest.raises(Stop, match="cuda:3"):
+        pipeline.infer(Matrix(), Rows(), [{}])
+    with pytest.raises(ValueError):
+        pipeline.infer(Matrix(), torch.zeros(3, 8), [{}])
