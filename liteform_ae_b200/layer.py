@@ -40,11 +40,11 @@ def _code(dtype, codes=_wide):
     """``LF_DTYPE_*`` of a torch type."""
     code = codes.get(dtype)
     if code is None:
-        if not _wide:
+        if not _wide:     # filled last, whole, so that another thread that finds it filled finds both
             torch = _torch()
-            _wide.update({torch.float32: _cabi.LF_DTYPE_F32, torch.bfloat16: _cabi.LF_DTYPE_BF16, torch.float16: _cabi.LF_DTYPE_F16})
-            _any.update(_wide)
-            _any[torch.float8_e4m3fn] = _cabi.LF_DTYPE_E4M3
+            wide = {torch.float32: _cabi.LF_DTYPE_F32, torch.bfloat16: _cabi.LF_DTYPE_BF16, torch.float16: _cabi.LF_DTYPE_F16}
+            _any.update({**wide, torch.float8_e4m3fn: _cabi.LF_DTYPE_E4M3})
+            _wide.update(wide)
             return _code(dtype, codes)
         raise ValueError(f"type {dtype} is not supported here")
     return code

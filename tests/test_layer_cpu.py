@@ -272,3 +272,35 @@ def test_infer_takes_the_matrix_to_its_rows(monkeypatch):
         pipeline.infer(Matrix(), Rows(), [{}])
     with pytest.raises(ValueError):
         pipeline.infer(Matrix(), torch.zeros(3, 8), [{}])
+
+
+def test_first_calls_of_two_threads(monkeypatch):
+    """The types are known to a call that comes at any line of another's first one."""
+    import sys
+    monkeypatch.setattr(layer, "_torch", lambda: torch)
+    monkeypatch.setattr(layer, "_wide", {})
+    monkeypatch.setattr(layer, "_any", {})
+    monkeypatch.setattr(layer._code, "__defaults__", (layer._wide,))
+    seen = []
+
+    def at_line(frame, event, arg):
+        if event == "line":
+            sys.settrace(None)      # the other thread's call, made here
+            held = [(d, dict(d)) for d in (layer._wide, layer._any)]
+            seen.append(layer._code(torch.float8_e4m3fn, layer._any))
+            assert layer._code(torch.float16) == _cabi.LF_DTYPE_F16
+            for d, before in held:  # as it was, for the lines that follow
+                d.clear()
+                d.update(before)
+            sys.settrace(trace)
+        return at_line
+
+    def trace(frame, event, arg):
+        return at_line if frame.f_code is layer._code.__code__ else None
+
+    sys.settrace(trace)
+    try:
+        assert layer._code(torch.float32) == _cabi.LF_DTYPE_F32
+    finally:
+        sys.settrace(None)
+    assert len(seen) > 5 and set(seen) == {E4M3}
