@@ -16,7 +16,8 @@ All computation is done by ``liblf_b200.so`` on torch's current stream of the te
 synchronised (except for a ``row_range``, see ``spmm_csr_act``).  The same call on the same inputs gives the same
 bits.  Matrices are dense in their last dimension and may have any row stride of at least their width; a row stride
 and address on 16-byte boundaries is faster.  Outputs may not share memory with each other or with inputs, but for the
-matrices that a call names as allowed.  ``ValueError`` for arguments that do not fit together.
+matrices that a call names as allowed.  Nothing is recorded for autograd: tensors that require a gradient are refused while
+gradients are enabled, the ``..._backward`` functions give them.  ``ValueError`` for arguments that do not fit together.
 """
 from __future__ import annotations
 
@@ -130,6 +131,15 @@ def _outputs_apart(given, inputs, may_be=()):
         seen.append((t, name, at))
 
 
+def _no_graph(*tensors):
+    """Refuses what autograd would lose without a word."""
+    if _torch().is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError("autograd does not see this call: make it under torch.no_grad(), or with detached tensors, and take "
+                                 "gradients from the ..._backward functions")
+
+
 def _act_code(activation):
     code = ACTIVATIONS.get(activation)
     if code is None:
@@ -194,6 +204,7 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, out_dtype=None, out=No
     scale per row (``y * scale`` is the row).  ``out``, ``scale``, ``sum_out`` and ``rstd`` take the outputs in place of new
     tensors; ``out`` and ``sum_out`` may each be ``x`` or ``residual`` itself."""
     torch = _torch()
+    _no_graph(x, weight, residual)
     if out is not None or sum_out is not None or scale is not None or rstd is not None:
         _outputs_apart(((out, "out"), (sum_out, "sum_out"), (scale, "scale"), (rstd, "rstd")),
                        ((x, "x"), (residual, "residual"), (weight, "weight")),
@@ -240,6 +251,7 @@ def rms_norm_backward(dy, h, weight, rstd, dh=None, dx=None, dweight=None, works
     float32.  For 8-bit rows pass the gradient of the rows they stand for (the rounding's own is taken as 1).
     ``dx`` may be ``dy``, ``h`` or ``dh``."""
     torch = _torch()
+    _no_graph(dy, h, weight, dh)
     if dx is not None or dweight is not None:
         _outputs_apart(((dx, "dx"), (dweight, "dweight")), ((dy, "dy"), (h, "h"), (dh, "dh"), (weight, "weight"), (rstd, "rstd")),
                        (("dx", "dy"), ("dx", "h"), ("dx", "dh"), ("dweight", "weight")))
@@ -335,6 +347,7 @@ def spmm_csr_act(a, B, scale=None, bias=None, activation: Optional[str] = None, 
     waits for the stream; a ``DeviceCsr`` of a slice of ``indptr`` does not.  Entries are not checked against B's rows:
     ``DeviceCsr.validate`` does that, once per matrix."""
     torch = _torch()
+    _no_graph(B, bias, residual, scale, values, None if isinstance(a, CsrTranspose) else a.data)
     if out is not None or preact is not None:
         _outputs_apart(((out, "out"), (preact, "preact")), ((B, "B"), (residual, "residual"), (bias, "bias"), (scale, "scale")),
                        (("out", "residual"), ("preact", "residual")))
@@ -383,6 +396,7 @@ def act_backward(dy, preact=None, activation: Optional[str] = None, dz=None, nee
     float32) and ``dbias`` the float32 sum of its rows before they are rounded; what is not needed is None.  ``dz`` may be
     ``dy`` or ``preact``."""
     torch = _torch()
+    _no_graph(dy, preact)
     if dz is not None or dbias is not None:
         _outputs_apart(((dz, "dz"), (dbias, "dbias")), ((dy, "dy"), (preact, "preact")), (("dz", "dy"), ("dz", "preact")))
     lib = _cabi.load()
@@ -415,6 +429,7 @@ def spmm_csr_grad_values(a: DeviceCsr, B, dy, preact=None, activation: Optional[
     ``dz = dy * activation'(preact)`` not rounded in between; float32, one per entry.  For a ``DeviceCsr`` of a slice of
     ``indptr`` the entries count from the slice's first, and what is behind its last is left as it is."""
     torch = _torch()
+    _no_graph(B, dy, preact)
     if out is not None:
         _outputs_apart(((out, "out"),), ((B, "B"), (dy, "dy"), (preact, "preact")))
     K, N, dev = _first(B, "B")

@@ -304,3 +304,13 @@ def test_first_calls_of_two_threads(monkeypatch):
     finally:
         sys.settrace(None)
     assert len(seen) > 5 and set(seen) == {E4M3}
+
+
+def test_tensors_that_require_a_gradient(monkeypatch):
+    monkeypatch.setattr(layer, "_torch", lambda: torch)
+    p, t = torch.zeros(3, requires_grad=True), torch.zeros(3)
+    layer._no_graph(t, None, p.detach())
+    with pytest.raises(ValueError, match="no_grad"):
+        layer._no_graph(t, None, p)
+    with torch.no_grad():
+        layer._no_graph(t, p)

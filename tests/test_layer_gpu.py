@@ -999,3 +999,22 @@ def test_act_backward_of_many_rows(cuda_device, M, N, extra, dtype, out, name):
     dz, db = layer.act_backward(dy, z, name, dz_dtype=out)
     ref.close(dz, want, ref.rounded(want, off, out), "dz")
     ref.close(db, want.sum(0), off.sum(0) + (M + 2) * U32 * (want.abs() + off).sum(0) + ref.TINY[F32], "dbias")
+
+
+def test_tensors_that_require_a_gradient_are_refused(cuda_device):
+    M, N = 20, 16
+    A = csr_on(cuda_device, pattern(M, M, 1), (M, M))
+    T = layer.CsrTranspose.of(A)
+    t, w, r = torch.randn(M, N, device=cuda_device), torch.ones(N, device=cuda_device), torch.ones(M, device=cuda_device)
+    p, q, v = t.clone().requires_grad_(), w.clone().requires_grad_(), A.data.clone().requires_grad_()
+    trained = hyb.DeviceCsr(A.indptr, A.indices, v, (M, M))
+    calls = [lambda: layer.rms_norm(p, w), lambda: layer.rms_norm(t, q), lambda: layer.rms_norm(t, w, residual=p),
+             lambda: layer.rms_norm_backward(p, t, w, r), lambda: layer.rms_norm_backward(t, t, q, r), lambda: layer.spmm_csr_act(A, p),
+             lambda: layer.spmm_csr_act(A, t, bias=q), lambda: layer.spmm_csr_act(A, t, residual=p), lambda: layer.spmm_csr_act(trained, t),
+             lambda: layer.spmm_csr_act(T, t, values=v), lambda: layer.act_backward(p), lambda: layer.act_backward(t, p, "silu"),
+             lambda: layer.spmm_csr_grad_values(A, p, t), lambda: layer.spmm_csr_act_backward(trained, T, t, t)]
+    for f in calls:
+        with pytest.raises(ValueError, match="no_grad"):
+            f()
+        with torch.no_grad():
+            f()
