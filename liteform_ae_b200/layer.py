@@ -314,6 +314,28 @@ class CsrTranspose:
         return CsrTranspose.from_host(csr.indptr.cpu().numpy(), csr.indices.cpu().numpy(), csr.shape, csr.indptr.device)
 
 
+    def validate(self, a: Optional[DeviceCsr] = None) -> None:
+        """``ValueError`` unless this is a pattern as ``DeviceCsr.validate`` wants it, with an ``order`` that names each entry once;
+        with ``a``, unless it is that matrix's.  ``from_host`` and ``of`` make such ones; arrays from elsewhere are not checked
+        by the products, which would read beside the values with a wrong ``order``.  Waits for the device."""
+        import torch
+        nnz, order = self.nnz, self.order
+        _need(order.dtype == torch.int32 and order.dim() == 1 and order.numel() == nnz, "order must be an int32 vector, one per entry")
+        if nnz:
+            _need(int(order.min()) >= 0 and int(order.max()) < nnz, "order must lie among the entries")
+            _need(int(torch.bincount(order, minlength=nnz).max()) == 1, "order must name each entry once")
+        if a is not None:
+            _need(a.shape == (self.shape[1], self.shape[0]) and a.nnz == nnz, "the pattern has another shape than the matrix transposed")
+        if 0 in self.shape:
+            _need(nnz == 0 and self.indptr.numel() == self.shape[0] + 1 and not bool(self.indptr.any()), "a matrix without rows or columns has no entries")
+            return
+        DeviceCsr(self.indptr, self.indices, None, self.shape).validate()
+        if a is not None:
+            rows = lambda ptr: torch.repeat_interleave(torch.arange(ptr.numel() - 1, device=ptr.device, dtype=torch.int32), torch.diff(ptr))
+            _need(bool((a.indices[order.long()] == rows(self.indptr)).all()) and bool((rows(a.indptr)[order.long()] == self.indices).all()),
+                  "the pattern is not that of the matrix transposed")
+
+
 def _csr_arrays(a, values, dev):
     """Addresses of the values and of their order."""
     transposed = isinstance(a, CsrTranspose)
@@ -345,7 +367,7 @@ def spmm_csr_act(a, B, scale=None, bias=None, activation: Optional[str] = None, 
     B's, bfloat16 for 8-bit rows); ``residual`` may be ``out``; ``preact`` (out's type) is filled with ``A @ B + bias`` for
     the backward pass.  ``row_range=(r0, r1)``: those rows of A only -- their number of entries is read back, which
     waits for the stream; a ``DeviceCsr`` of a slice of ``indptr`` does not.  Entries are not checked against B's rows:
-    ``DeviceCsr.validate`` does that, once per matrix."""
+    ``DeviceCsr.validate`` does that, once per matrix (``CsrTranspose.validate`` also for ``order``)."""
     torch = _torch()
     _no_graph(B, bias, residual, scale, values, None if isinstance(a, CsrTranspose) else a.data)
     if out is not None or preact is not None:

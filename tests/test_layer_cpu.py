@@ -314,3 +314,21 @@ def test_tensors_that_require_a_gradient(monkeypatch):
         layer._no_graph(t, None, p)
     with torch.no_grad():
         layer._no_graph(t, p)
+
+
+@pytest.mark.parametrize("order", [[0, 1, 2, 3], [0, 1, 2, 3, 5], [0, 1, 2, 3, -1], [0, 1, 2, 3, 3], [0, 4, 4, 3, 2]])
+def test_orders_that_are_none(order):
+    t = layer.CsrTranspose.from_host(np.array([0, 2, 5]), np.array([0, 3, 0, 1, 2]), (2, 4), "cpu")
+    t.order = torch.tensor(order, dtype=torch.int32)
+    with pytest.raises(ValueError, match="order"):
+        t.validate()
+
+
+def test_order_of_another_type_or_matrix():
+    from liteform_ae_b200 import hyb
+    t = layer.CsrTranspose.from_host(np.array([0, 2, 5]), np.array([0, 3, 0, 1, 2]), (2, 4), "cpu")
+    with pytest.raises(ValueError, match="shape"):
+        t.validate(hyb.DeviceCsr(torch.tensor([0, 2, 5]), torch.zeros(5, dtype=torch.int32), None, (2, 5)))
+    t.order = t.order.long()
+    with pytest.raises(ValueError, match="order"):
+        t.validate()

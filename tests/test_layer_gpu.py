@@ -1018,3 +1018,23 @@ def test_tensors_that_require_a_gradient_are_refused(cuda_device):
             f()
         with torch.no_grad():
             f()
+
+
+def test_transposed_patterns_are_validated(cuda_device):
+    for M, K in ((40, 30), (1, 50), (30, 1), (5, 0), (0, 5)):
+        A = csr_on(cuda_device, pattern(M, K, 3) if M and K else (torch.zeros(M + 1, dtype=torch.int64), torch.empty(0, dtype=torch.int32), torch.empty(0)), (M, K))
+        T = layer.CsrTranspose.of(A)
+        T.validate()
+        T.validate(A)
+    A = csr_on(cuda_device, pattern(40, 30, 3), (40, 30))
+    T = layer.CsrTranspose.of(A)
+    other = csr_on(cuda_device, pattern(40, 30, 3), (40, 30))
+    other.indices = (29 - other.indices)      # as many entries, elsewhere
+    swapped = T.order.clone()
+    swapped[:2] = T.order[:2].flip(0)
+    far = T.indices.clone()
+    far[-1] = 40
+    for t, a in ((T, other), (layer.CsrTranspose(T.indptr, T.indices, swapped, T.shape), A), (layer.CsrTranspose(T.indptr, far, T.order, T.shape), None),
+                 (layer.CsrTranspose(T.indptr, T.indices, T.order, (30, 39)), A), (layer.CsrTranspose(T.indptr.flip(0), T.indices, T.order, T.shape), None)):
+        with pytest.raises(ValueError):
+            t.validate(a)
