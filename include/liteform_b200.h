@@ -417,8 +417,9 @@ int lf_shard_rows(const int64_t* indptr /*[dev]*/, int64_t num_rows, int32_t num
  * Types are LF_DTYPE_*; LF_DTYPE_E4M3 is the 8-bit float with 4 exponent and 3 mantissa bits (no
  * infinity, largest value 448), always with one float32 scale per row: the row stands for
  * scale * its stored values.  Sums, statistics and activations are float32, every output is
- * rounded once, to nearest even.  Strides (ld...) are in elements; rows may start anywhere their
- * element type allows, but rows on 16-byte boundaries (address and stride) move faster.  Results
+ * rounded once, to nearest even.  Strides (ld...) are in elements; rows may start at any multiple of
+ * their element's size (other addresses are refused), but rows on 16-byte boundaries (address and
+ * stride) move faster.  Results
  * do not depend on the order in which thread blocks run: the same call gives the same bits.
  * ------------------------------------------------------------------------------------------- */
 #define LF_DTYPE_E4M3 3

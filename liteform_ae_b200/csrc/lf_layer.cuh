@@ -13,6 +13,9 @@ namespace lf {
 
 inline bool is_wide_dtype(int32_t dt) { return dt == LF_DTYPE_F32 || dt == LF_DTYPE_BF16 || dt == LF_DTYPE_F16; }
 __host__ __device__ inline int dtype_bytes(int32_t dt) { return dt == LF_DTYPE_F32 ? 4 : dt == LF_DTYPE_E4M3 ? 1 : 2; }
+// what a misaligned address would fault on; NULL is aligned
+inline bool aligned(const void* p, int bytes) { return (uintptr_t)p % bytes == 0; }
+inline bool aligned_for(const void* p, int32_t dt) { return aligned(p, dtype_bytes(dt)); }
 inline bool on_grid16(const void* p, int64_t ld, int32_t dt) {   // every row starts on a 16-byte boundary
   return (uintptr_t)p % 16 == 0 && ld * dtype_bytes(dt) % 16 == 0;
 }

@@ -517,6 +517,9 @@ int lf_rms_norm(const void* x, int32_t dtype, int64_t ld_x, const void* residual
   LF_REQUIRE(x && weight && y, "null pointer argument");
   LF_REQUIRE(!residual || (sum && ld_residual >= N && ld_sum >= N), "a residual needs a place for the sum");
   LF_REQUIRE(y_dtype != LF_DTYPE_E4M3 || scale, "8-bit rows need a place for their scales");
+  LF_REQUIRE(aligned_for(x, dtype) && aligned_for(residual, dtype) && (!residual || aligned_for(sum, dtype)) && aligned_for(weight, weight_dtype) &&
+                 aligned_for(y, y_dtype) && (y_dtype != LF_DTYPE_E4M3 || aligned(scale, 4)) && aligned(rstd, 4),
+             "an address is not a multiple of its type's size");
   const NormArgs a{x, residual, weight, sum, y, scale, rstd, rows, ld_x, ld_residual, ld_sum, ld_y, N, weight_dtype, y_dtype, eps};
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == LF_DTYPE_F32) LF_CUDA_CHECK(launch_norm<LF_DTYPE_F32>(a, st));
@@ -544,6 +547,9 @@ int lf_rms_norm_backward(const void* dy, int64_t ld_dy, const void* h, int64_t l
   }
   LF_REQUIRE(dy && h && weight && rstd && dx, "null pointer argument");
   LF_REQUIRE(ld_dy >= N && ld_h >= N && ld_dx >= N && (!dsum || ld_dsum >= N), "bad leading dimension");
+  LF_REQUIRE(aligned_for(dy, dtype) && aligned_for(h, dtype) && aligned_for(dsum, dtype) && aligned_for(dx, dtype) && aligned_for(weight, weight_dtype) &&
+                 aligned(rstd, 4) && aligned(dweight, 4) && aligned(workspace, 4),
+             "an address is not a multiple of its type's size");
   if (workspace_bytes < lf_rms_norm_backward_workspace_bytes(rows, N) || !workspace)
     return fail(LF_ERR_WORKSPACE_TOO_SMALL, "workspace of %zu bytes, %zu needed", workspace_bytes,
                 lf_rms_norm_backward_workspace_bytes(rows, N));

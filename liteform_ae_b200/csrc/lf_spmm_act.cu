@@ -394,6 +394,9 @@ int lf_spmm_csr_act(const int64_t* indptr, const int32_t* indices, const float* 
   if (row_begin == row_end) return LF_OK;
   LF_REQUIRE(indptr && C, "null pointer argument");
   LF_REQUIRE(nnz == 0 || (indices && B), "indices or B missing");
+  LF_REQUIRE(aligned(indptr, 8) && aligned(indices, 4) && aligned(data, 4) && aligned(order, 4) && aligned(b_scale, 4) && aligned_for(B, b_dtype) &&
+                 aligned_for(C, c_dtype) && aligned_for(ep.bias, ep.bias_dtype) && aligned_for(ep.residual, ep.residual_dtype) && aligned_for(ep.preact, c_dtype),
+             "an address is not a multiple of its type's size");
   LF_REQUIRE(!order || (data && nnz < (1ll << 31)), "order goes with data, for fewer than 2^31 entries");
   const size_t need = lf_spmm_csr_act_workspace_bytes(nnz, N, b_dtype);
   if (need > 0 && (!workspace || workspace_bytes < need))

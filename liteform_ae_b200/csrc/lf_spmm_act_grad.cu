@@ -305,6 +305,9 @@ int lf_act_backward_as(const void* dy, int64_t ld_dy, const void* preact, int64_
   }
   LF_REQUIRE(dy && (preact || activation == LF_ACT_NONE), "null pointer argument");
   LF_REQUIRE(ld_dy >= N && (activation == LF_ACT_NONE || ld_preact >= N) && (!dz || ld_dz >= N), "bad leading dimension");
+  LF_REQUIRE(aligned_for(dy, dtype) && (activation == LF_ACT_NONE || aligned_for(preact, dtype)) && aligned_for(dz, dz_dtype) && aligned(dbias, 4) &&
+                 (!dbias || aligned(workspace, 4)),
+             "an address is not a multiple of its type's size");
   if (dbias && (!workspace || workspace_bytes < lf_act_backward_workspace_bytes(rows, N)))
     return fail(LF_ERR_WORKSPACE_TOO_SMALL, "workspace of %zu bytes, %zu needed", workspace_bytes,
                 lf_act_backward_workspace_bytes(rows, N));
@@ -345,6 +348,9 @@ int lf_spmm_csr_grad_values(const int64_t* indptr, const int32_t* indices, int64
   if (row_begin == row_end || nnz == 0) return LF_OK;
   LF_REQUIRE(indptr && indices && dy && B && dvalues, "null pointer argument");
   LF_REQUIRE(activation == LF_ACT_NONE || (preact && ld_preact >= N && ld_preact < (1ll << 30)), "preact missing");
+  LF_REQUIRE(aligned(indptr, 8) && aligned(indices, 4) && aligned(dvalues, 4) && aligned_for(dy, dy_dtype) &&
+                 (activation == LF_ACT_NONE || aligned_for(preact, dy_dtype)) && aligned_for(B, b_dtype),
+             "an address is not a multiple of its type's size");
   const int lg = range_log(nnz, row_end - row_begin);
   LF_REQUIRE((nnz >> lg) < (1ll << 31) - 1, "too many entries");
   const uint32_t bytes = (uint32_t)dtype_bytes(dy_dtype);

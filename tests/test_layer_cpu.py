@@ -332,3 +332,24 @@ def test_order_of_another_type_or_matrix():
     t.order = t.order.long()
     with pytest.raises(ValueError, match="order"):
         t.validate()
+
+
+R8 = dict(res=P, ld_res=8, sum=P, ld_sum=8)
+EP = dict(residual=2 * P, residual_dtype=F32, ld_residual=8, bias=P, bias_dtype=F32, preact=3 * P, ld_preact=8)
+
+
+@pytest.mark.parametrize("call, kw", [(norm, dict(x=P + 2)), (norm, dict(w=P + 1)), (norm, dict(y=P + 2)), (norm, dict(rstd=P + 2)),
+                                      (norm, dict(yd=E4M3, scale=P + 1)), (norm, dict(R8, res=P + 2)), (norm, dict(R8, sum=P + 3)),
+                                      (norm, dict(dtype=BF16, x=P + 1)), (norm_grad, dict(dy=P + 2)), (norm_grad, dict(h=P + 1)),
+                                      (norm_grad, dict(w=P + 2)), (norm_grad, dict(rstd=P + 2)), (norm_grad, dict(ds=P + 2, ld_ds=8)),
+                                      (norm_grad, dict(dx=P + 2)), (norm_grad, dict(dw=P + 2)), (norm_grad, dict(ws=P + 2)),
+                                      (product, dict(indptr=P + 4)), (product, dict(indices=P + 2)), (product, dict(data=P + 2)),
+                                      (product, dict(order=P + 2)), (product, dict(B=P + 2)), (product, dict(C=2 * P + 2)), (product, dict(scale=P + 2)),
+                                      (product, dict(bd=BF16, B=P + 1)), (product, dict(C=4 * P, ep=dict(EP, bias=P + 2))),
+                                      (product, dict(C=4 * P, ep=dict(EP, residual=P + 2))), (product, dict(C=4 * P, ep=dict(EP, preact=P + 2))),
+                                      (act_grad, dict(dy=P + 2)), (act_grad, dict(z=P + 2)), (act_grad, dict(dz=P + 2)), (act_grad, dict(db=P + 2)),
+                                      (act_grad, dict(ws=P + 2)), (act_grad_as, dict(dz=P + 2)), (act_grad_as, dict(dy=P + 1)),
+                                      (value_grad, dict(indptr=P + 4)), (value_grad, dict(indices=P + 2)), (value_grad, dict(dy=P + 2)),
+                                      (value_grad, dict(z=P + 2)), (value_grad, dict(B=P + 2)), (value_grad, dict(dv=P + 2))])
+def test_addresses_off_their_type(call, kw):
+    assert call(**(dict(dict(C=4 * P), **kw) if call is product else kw)) == BAD and b"multiple" in _cabi.load().lf_last_error()
