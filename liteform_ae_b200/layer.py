@@ -159,11 +159,12 @@ def _run(fn, call, dev):
 
 
 def _scratch(nbytes, workspace, like):
-    """``(buffer, address, size)`` of ``nbytes`` on the device of ``like``; the buffer has to outlive the call."""
+    """``(buffer, address, size)`` of ``nbytes`` on the device of ``like``; the buffer has to outlive the call.  A call that is
+    captured takes memory of its graph's own: a workspace may grow, and its old buffer be another tensor's by the replay."""
     if nbytes == 0:
         return None, 0, 0
     torch = _torch()
-    if workspace is None:
+    if workspace is None or torch.cuda.is_current_stream_capturing():
         buf = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
     else:
         buf = workspace.get(nbytes)

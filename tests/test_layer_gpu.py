@@ -1038,3 +1038,51 @@ def test_transposed_patterns_are_validated(cuda_device):
                  (layer.CsrTranspose(T.indptr, T.indices, T.order, (30, 39)), A), (layer.CsrTranspose(T.indptr.flip(0), T.indices, T.order, T.shape), None)):
         with pytest.raises(ValueError):
             t.validate(a)
+
+
+def test_captured_calls_leave_the_workspace_alone(cuda_device):
+    """A workspace that has grown since the capture is no part of the replay."""
+    g = gen(8)
+    M, K, N = 300, 2500, 96
+    A = csr_on(cuda_device, pattern(M, K, 9, 12.0, 2500), (M, K))
+    B, dy = torch.randn(K, N, generator=g).to(cuda_device), torch.randn(M, N, generator=g).to(cuda_device)
+    h, w, r = torch.randn(M, N, generator=g).to(cuda_device), torch.ones(N, device=cuda_device), torch.ones(M, device=cuda_device)
+    ws = hyb.Workspace(cuda_device)
+    step = lambda: (layer.spmm_csr_act(A, B, workspace=ws), *layer.act_backward(dy, dy, "silu", workspace=ws),
+                    *layer.rms_norm_backward(dy, h, w, r, workspace=ws))
+    want = [t.clone() for t in step()]
+    held = ws._buf
+    assert held is not None and held.numel() >= 1000
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    assert ws._buf is held
+    held.fill_(0x5a)            # as if it were another tensor's by now
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(out, want)) and bool((held == 0x5a).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, E4M3])
+@pytest.mark.parametrize("N", [64, 33])
+def test_scales_of_any_type_and_ranges_of_a_transposed_pattern(cuda_device, dtype, N):
+    g = gen(N)
+    M, K = 150, 110
+    p = pattern(M, K, 4, 9.0, 110)
+    A = csr_on(cuda_device, p, (M, K))
+    T = layer.CsrTranspose.of(A)
+    a = ref.dense(*p, (M, K))
+    for m, at, rows, ad in ((A, None, K, a), (T, A.data, M, a.t().contiguous())):
+        B, _, Bv = features(rows, N, F32 if dtype == E4M3 else dtype, g, cuda_device)
+        if dtype == E4M3:
+            B, Bv = B.to(E4M3), B.to(E4M3).cpu().double()
+        s = torch.rand(rows, generator=g) * 2 - 1
+        n = ad.shape[0]
+        R, Rv = rows_of((n, N), F32, g, cuda_device)
+        z, y, zoff, yoff = ref.product(ad, Bv * s.double()[:, None], None, "silu", Rv, F32)
+        kw = dict(scale=s.to(cuda_device), activation="silu", values=at, out_dtype=F32)
+        ref.close(layer.spmm_csr_act(m, B, residual=R, **kw), y, yoff)
+        for r0, r1 in ((0, 1), (37, 90), (n - 1, n), (50, 50)):
+            pre = torch.empty(r1 - r0, N, device=cuda_device)
+            ref.close(layer.spmm_csr_act(m, B, residual=R[r0:r1], preact=pre, row_range=(r0, r1), **kw), y[r0:r1], yoff[r0:r1], (r0, r1))
+            ref.close(pre, z[r0:r1], zoff[r0:r1], (r0, r1))
