@@ -448,7 +448,7 @@ typedef struct lf_epilogue {
  * data[order[e]] -- A transposed, given by its own indptr and indices, over the values of A.  An
  * entry whose value is 0 reads nothing of B (nor its scale), so it passes on no NaN or infinity.
  * nnz: the exact number of entries of the rows, for the workspace's size too (it does not grow
- * steadily).  The workspace holds the sums of rows that several thread groups share; it may be used
+ * steadily, and is the same for every b_dtype).  The workspace holds the sums of rows that several thread groups share; it may be used
  * again as soon as the call is over on the stream, not by two calls at a time.  C and preact must not
  * share memory with B or with each other, nor with a residual that is not the same rows: equal addresses
  * are refused, other overlaps are the caller's to avoid (the Python calls compare the ranges).  Fewer than 2^31 rows, every stride below 2^30, at most 2^22 features.

@@ -11,6 +11,7 @@
 
 namespace lf {
 
+constexpr int kSms = 148;   // of a B200: launches are sized by it, and workspaces, whose sizes are asked for without a device
 inline bool is_wide_dtype(int32_t dt) { return dt == LF_DTYPE_F32 || dt == LF_DTYPE_BF16 || dt == LF_DTYPE_F16; }
 __host__ __device__ inline int dtype_bytes(int32_t dt) { return dt == LF_DTYPE_F32 ? 4 : dt == LF_DTYPE_E4M3 ? 1 : 2; }
 // what a misaligned address would fault on; NULL is aligned
@@ -58,15 +59,6 @@ struct Pack {
     uint8_t b;
   };
   __device__ __forceinline__ Pack() {}
-  __device__ __forceinline__ void load(const void* p) {
-    if constexpr (kWord == 16) {
-#pragma unroll
-      for (int i = 0; i < kBytes / 16; ++i) q[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-    } else if constexpr (kWord == 8) d = __ldg(reinterpret_cast<const uint2*>(p));
-    else if constexpr (kWord == 4) w = __ldg(reinterpret_cast<const uint32_t*>(p));
-    else if constexpr (kWord == 2) h = __ldg(reinterpret_cast<const uint16_t*>(p));
-    else b = __ldg(reinterpret_cast<const uint8_t*>(p));
-  }
   __device__ __forceinline__ void fetch(const void* p) {   // read once, by the thread that may write there later: streaming
     if constexpr (kWord == 16) {
 #pragma unroll

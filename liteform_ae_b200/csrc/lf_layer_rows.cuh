@@ -9,9 +9,9 @@
 // Why sorted rows: graphs have most of their rows at a few entries and most of their entries in a few rows.  Groups that
 // end their rows at different steps run the epilogue one after the other; rows of about one length end together, and
 // nothing has to notice where a row ends.  2^20 power-law rows, 13.2 M entries, 128 bfloat16 features, bias, relu and
-// residual: groups that walk over entries at an even pace, finished rows in a queue, 985 us; thread blocks that stage row
-// starts in the place of entries 1193; sorted rows with four gathers per group in registers instead of the ring 1441; as
-// it stands 563.
+// residual (the graph below): groups that walk over entries at an even pace, finished rows in a queue, 985 us; thread blocks
+// that stage row starts in the place of entries 1193; sorted rows with four gathers per group in registers instead of the ring
+// 1441; the first form with the ring 624; now 555, both launches.  Figures of a choice beside others were taken when it was made.
 #pragma once
 
 #include "lf_layer.cuh"
@@ -19,13 +19,13 @@
 
 namespace lf {
 
-// Entries of a warp's range: the most that still gives each of the chip's 148 SMs the 20 warps that it could hold, three times
+// Entries of a warp's range: the most that still gives each SM 20 warps (it holds 17 to 19 at a time), three times
 // over where there are enough, from 64 to 2048 (2^20 uniform rows, 33.5 M entries: 735 us with 1024 each, 707 with 2048; the
-// power-law rows above 620 with 512, 615 with 1024).  From 16 where most rows have no entry, since there each may take a search
+// graph above 620 with 512, 615 with 1024).  From 16 where most rows have no entry, since there each may take a search
 // for its row (332 469 rows with 40 entries: 196 us for 64, 85 for 16; 3497 rows with 56 000, some of them long: 27 and 34).
 inline int range_log(int64_t nnz, int64_t rows) {
   int lg = 11;
-  while (lg > (rows > nnz ? 4 : 6) && (nnz >> lg) < 148 * 20 * (lg > 8 ? 3 : 1)) --lg;
+  while (lg > (rows > nnz ? 4 : 6) && (nnz >> lg) < kSms * 20 * (lg > 8 ? 3 : 1)) --lg;
   return lg;
 }
 // A row that starts in a range and ends at most so far behind its nominal end belongs to it whole; only longer ones are
@@ -238,9 +238,12 @@ struct WalkArgs {
 };
 
 constexpr int kWalkThreads = 32;    // a warp: a block of two keeps its place until the slower is done (589 us on the graph above for 561)
-constexpr int kWalkBlocks = 17;     // per SM that the registers have to allow (shared memory: 19).  16: 614 us, 17: 563, 18: 560, 20: 585; the same in 8 bits: 712, 633, 642, 655
+// Blocks per SM that the registers have to allow; shared memory allows 17 to 19 with the span of the bias.  16 are four to each of
+// the SM's register files, so 128 registers; 17 to 20 are five, so 96 without spills, but the compiler orders instructions for the
+// number it is given.  16, 17, 18, 20: 588, 558, 560, 563 us on the graph above, in 8 bits 651, 584, 607, 613.
+constexpr int kWalkBlocks = 17;
 constexpr int kWindow = 256;        // entries of the rows taken at a time, rows rounded up to fours
-constexpr int kShortRow = 64;       // longest row that one group does (16 / 32 / 64 / 128: 713 / 622 / 606 / 642 us on the graph above)
+constexpr int kShortRow = 64;       // longest row that one group does (16 / 32 / 64 / 128: 713 / 622 / 606 / 642 us on the graph above, in an earlier form)
 constexpr int kAtOnce = 4;          // steps (a row of B per group) that are copied and added up together
 constexpr int kRingBytes = 8192;
 constexpr uint32_t kNothing = 0x80000000u;   // mark of a column whose row of B is not read

@@ -297,7 +297,10 @@ rms_norm_grad_rows_kernel(NormGradArgs a) {
 }
 
 // Blocks of the gradient's kernel that an SM holds at a time; the launch has as many, since each walks over an equal
-// share of the rows (2^18 rows of 512 bfloat16: 3 held and 592 launched 236 us, 444 181: 5.9 TB/s).
+// share of the rows (2^18 rows of 512 bfloat16: 3 held and 592 launched 236 us, 444 181: 5.9 TB/s).  Wider rows have one, and nothing
+// on its way between a row's two barriers: 2^15 rows of 4096 bfloat16 335 us where the bytes take 164; 257 to 512 float32
+// features spill (2^18 rows of 384: 360 us for 246), and rows off the grid beyond 4096 go element by element, their sums in
+// memory (2^14 rows of 4099 bfloat16: 845 us for 82).
 template <int VEC, int L, int C> constexpr int kGradResident = L <= 256 && C * VEC <= 16 ? 3 : 1;
 
 // The same for the gradients, row after row; the weight's is summed over the rows that a thread sees, then over the groups of its
@@ -425,7 +428,7 @@ cudaError_t launch_column_sum(const float* partial, int parts, int N, float* out
 
 namespace {
 
-constexpr int kSms = 148, kNormGradBlocks = 3 * kSms;
+constexpr int kNormGradBlocks = 3 * kSms;
 
 inline bool rows_on(const void* p, int64_t ld, int bytes, int grid) { return (uintptr_t)p % grid == 0 && ld * bytes % grid == 0; }
 

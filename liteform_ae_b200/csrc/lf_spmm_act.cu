@@ -2,8 +2,8 @@
 //
 // What it has to move: the entries (8 bytes each), C and the residual once; what bounds it are the rows of B, one for each
 // entry, out of the L2 and, as far as B is larger than that, out of memory, and the instructions that unpack and add them.
-// 2^20 power-law rows with 13.2 M entries: 128 bfloat16 features 0.55 ms (3.4 GB of rows of B, 6.2 TB/s), the same in 8 bits
-// 0.58 ms; the entries, one read of B and C and the residual would take 0.14 and 0.12 ms.
+// 2^20 power-law rows with 13.2 M entries: 128 bfloat16 features 555 us (3.4 GB of rows of B, 6.1 TB/s), the same in 8 bits
+// 584; the entries, one read of B and C and the residual would take 0.14 and 0.12 ms.
 //
 // Two launches.  In the first a warp takes a range of entries and does the rows in it (lf_layer_rows.cuh); a group of
 // lanes that has summed up its row runs the epilogue on its registers, the residual having been fetched along with the rows
@@ -128,8 +128,8 @@ __device__ __forceinline__ void finish8(const ActArgs& a, int row, int f, const 
 }
 
 // ---- the walk ---------------------------------------------------------------------------------------
-// What is known of C, residual and preact when the kernel is compiled (2^20 power-law rows, 128 bfloat16 features 566 us with
-// kAnyRows, 551 with kOnGrid, 540 with kTyped; in 8 bits 595 and 579 with the latter two; 2^20 uniform rows of 64 features in 8
+// What is known of C, residual and preact when the kernel is compiled (the first launch alone, 2^20 power-law rows, 128 bfloat16
+// features: 566 us with kAnyRows, 551 with kOnGrid, 540 with kTyped; in 8 bits 595 and 579 with the latter two; 2^20 uniform rows of 64 features in 8
 // bits 790 with the first and 724 with the second).  Other types than kTyped's are compiled for the grid only from 8 bits, where
 // there is no type of its own for C.
 enum Rows { kAnyRows, kOnGrid, kTyped };   // on the grid: on 16-byte boundaries and of whole pieces; typed: of kOwn as well
@@ -236,7 +236,9 @@ spmm_csr_act_kernel(const __grid_constant__ ActArgs a) {
 
 // Rows without entries, and rows that several ranges share: their pieces in order.  Most of its time goes into looking
 // at row pointers (2^20 rows: 16 us).  A lane has eight features; rows of few pieces
-// are a warp's, rows of many the block's, whose warps take every eighth piece.
+// are a warp's, rows of many the block's, whose warps take every eighth piece.  Six blocks an SM, for the looking, leave 40 registers:
+// the epilogue and the adding up spill (308 bytes), and act(bias) is computed for every row without entries.  Those are written at
+// 3.3 TB/s.
 constexpr int kLongPieces = 8;
 
 __device__ __forceinline__ void bias8(const ActArgs& a, int f, float* b) {
@@ -422,7 +424,7 @@ int lf_spmm_csr_act(const int64_t* indptr, const int32_t* indices, const float* 
   // few rows per block while that fills the chip: a block's long rows are done one after the other (16384 rows, 64 of them
   // with 2048 entries: 35 us with 256 rows a block, 17 with 32)
   int span = 32;
-  while (span < kThreads && a.rows > (int64_t)span * 148 * 8) span *= 2;
+  while (span < kThreads && a.rows > (int64_t)span * kSms * 8) span *= 2;
   const int64_t blocks = ceil_div64(a.rows, span);
   LF_CUDA_CHECK(launch_dep(finish_rows_kernel, dim3((unsigned)(blocks < (1 << 16) ? blocks : 1 << 16)), kThreads, st, nnz > 0, a, span));
   return LF_OK;

@@ -22,9 +22,9 @@ struct ActGradArgs {
 };
 
 // A block's threads are 256 / per_row rows side by side, VEC features each; a thread keeps its features while it walks down
-// the rows, so that the bias's sum stays in registers.  The inputs are read once and dZ is written once: memory bounds it,
-// and, with the error function's slope, the special functions (2^18 rows of 256 bfloat16, gelu: 91 us, 4.4 TB/s; the bytes
-// alone would take 61).
+// the rows, so that the bias's sum stays in registers.  The inputs are read once and dZ is written once (61 us for 2^18 rows
+// of 256 bfloat16).  Under the profiler relu takes 79 us, waiting for loads with half of an SM's warps, and gelu 99, issuing in
+// 67 % of the cycles.  48 registers leave five blocks an SM, and the launch has six for each: the last one runs alone.
 template <int DT, int OUT, int VEC>   // of dy and z, of dz
 __global__ void __launch_bounds__(256)
 act_grad_kernel(ActGradArgs a) {
@@ -70,7 +70,7 @@ act_grad_kernel(ActGradArgs a) {
   }
 }
 
-constexpr int kMostParts = 148 * 6;
+constexpr int kMostParts = kSms * 6;
 
 // ---- gradient of the values -------------------------------------------------------------------------
 struct ValueGradArgs {
@@ -89,7 +89,8 @@ struct ValueGradArgs {
 // The group keeps its row of dZ in registers (computed there, not rounded) and multiplies the rows of B that come through the
 // ring with it; four dot products at a time are summed up over the lanes, each lane ending with one of them.  A row wider
 // than a walk takes several launches, which add to what the ones before wrote.  As in the product, the rows of B and the
-// instructions on them bound it (2^18 power-law rows, 3.1 M entries, 256 bfloat16 features, gelu: 300 us).
+// instructions on them bound it (2^18 power-law rows, 3.1 M entries, 256 bfloat16 features, gelu: 302 us, instructions in 71 % of the
+// cycles).
 // VIO: rows of dy and z have B's type and are known to be on the grid.
 template <int DT, int G, int CH, bool VIO>
 struct GradWork {
