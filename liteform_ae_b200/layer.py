@@ -314,7 +314,6 @@ class CsrTranspose:
         """From a matrix in device memory (sorted on the host: done once per matrix)."""
         return CsrTranspose.from_host(csr.indptr.cpu().numpy(), csr.indices.cpu().numpy(), csr.shape, csr.indptr.device)
 
-
     def validate(self, a: Optional[DeviceCsr] = None) -> None:
         """``ValueError`` unless this is a pattern as ``DeviceCsr.validate`` wants it, with an ``order`` that names each entry once;
         with ``a``, unless it is that matrix's.  ``from_host`` and ``of`` make such ones; arrays from elsewhere are not checked
@@ -327,6 +326,9 @@ class CsrTranspose:
             _need(int(torch.bincount(order, minlength=nnz).max()) == 1, "order must name each entry once")
         if a is not None:
             _need(a.shape == (self.shape[1], self.shape[0]) and a.nnz == nnz, "the pattern has another shape than the matrix transposed")
+        for t, dtype, name in ((self.indptr, torch.int64, "indptr"), (self.indices, torch.int32, "indices")):
+            _need(t.dtype == dtype and t.dim() == 1 and t.is_contiguous() and t.device == order.device, f"{name} must be a dense {dtype} vector beside order")
+        _need(self.indptr.numel() == self.shape[0] + 1, "indptr must have one more than the rows")
         if 0 in self.shape:
             _need(nnz == 0 and self.indptr.numel() == self.shape[0] + 1 and not bool(self.indptr.any()), "a matrix without rows or columns has no entries")
             return

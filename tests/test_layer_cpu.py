@@ -353,3 +353,13 @@ EP = dict(residual=2 * P, residual_dtype=F32, ld_residual=8, bias=P, bias_dtype=
                                       (value_grad, dict(z=P + 2)), (value_grad, dict(B=P + 2)), (value_grad, dict(dv=P + 2))])
 def test_addresses_off_their_type(call, kw):
     assert call(**(dict(dict(C=4 * P), **kw) if call is product else kw)) == BAD and b"multiple" in _cabi.load().lf_last_error()
+
+
+@pytest.mark.parametrize("change", [dict(indptr=torch.int32), dict(indices=torch.int64), dict(indptr=torch.float64), dict(shape=(5, 2)), dict(shape=(3, 2))])
+def test_patterns_of_other_types_or_sizes(change):
+    """Refused before anything reads them as what they are not."""
+    t = layer.CsrTranspose.from_host(np.array([0, 2, 5]), np.array([0, 3, 0, 1, 2]), (2, 4), "cpu")
+    for name, to in change.items():
+        setattr(t, name, to if name == "shape" else getattr(t, name).to(to))
+    with pytest.raises(ValueError, match="ind"):
+        t.validate()
